@@ -18,7 +18,7 @@ engine drives the same pipeline imperatively per step:
 
 Learning-rate schedules (fixed / polynomial / exponential) and the optimizer
 set (adadelta / adagrad / adam / rmsprop / sgd) mirror graph.py:51-66 with
-the same sub-argument names and defaults.
+the same sub-argument names and defaults; adamw is this framework's own.
 """
 
 import torch
@@ -26,6 +26,7 @@ import torch
 from . import aggregators as aggregators_mod
 from . import attacks as attacks_mod
 from . import config, tools
+from .optim import AdamW
 
 # ---------------------------------------------------------------------------- #
 # Learning-rate schedules (reference graph.py:51-57)
@@ -72,6 +73,18 @@ optimizers = {
         "args": {"adam-beta1": 0.9, "adam-beta2": 0.999},
         "fn": lambda params, lr, a: torch.optim.Adam(
             params, lr=lr, betas=(a["adam-beta1"], a["adam-beta2"])),
+    },
+    # Not the reference's: decoupled weight decay, states in 32 or 8 bits and
+    # clipping by the global norm, on the framework's own kernels.
+    "adamw": {
+        "args": {"adam-beta1": 0.9, "adam-beta2": 0.999, "opt-epsilon": 1e-8,
+                 "weight-decay": 1e-2, "clip-norm": -1., "state-bits": 32,
+                 "rounding-seed": 0},
+        "fn": lambda params, lr, a: AdamW(
+            params, lr=lr, betas=(a["adam-beta1"], a["adam-beta2"]),
+            eps=a["opt-epsilon"], weight_decay=a["weight-decay"],
+            state_bits=a["state-bits"], rounding_seed=a["rounding-seed"],
+            max_norm=a["clip-norm"] if a["clip-norm"] > 0 else None),
     },
     "rmsprop": {
         "args": {},

@@ -1,7 +1,8 @@
-"""GAR compute ops: HIP/CDNA4 kernels on GPU, PyTorch oracle on CPU.
+"""Compute ops: HIP/CDNA4 kernels on GPU, PyTorch oracle on CPU.
 
-Every public function takes the stacked ``[n, d]`` gradient matrix and
-dispatches on its device:
+Every GAR function takes the stacked ``[n, d]`` gradient matrix, every
+optimizer function (:mod:`aggregathor_amd.ops.adamw`) lists of tensors; both
+dispatch on the device:
 
 - CUDA (= ROCm/HIP) tensors run the hand-written gfx950 kernels from the
   in-tree ``_gar_hip`` torch extension (``aggregathor_amd/ops/csrc``). If the
@@ -11,8 +12,9 @@ dispatches on its device:
   TF silently placing kernels on CPU cost "two orders of magnitude",
   /root/reference/README.md:174-182).
 - CPU tensors run the pure-PyTorch reference implementations
-  (:mod:`aggregathor_amd.ops.reference`), which are also the numerics oracle
-  for the HIP kernels.
+  (:mod:`aggregathor_amd.ops.reference`,
+  :mod:`aggregathor_amd.ops.adamw_reference`), which are also the numerics
+  oracle for the HIP kernels.
 
 Set ``AGGREGATHOR_FORCE_EAGER=1`` to force the PyTorch path on GPU (debug
 only; benchmarks refuse it).
@@ -126,3 +128,10 @@ def bulyan(grads, f, m=None):
     if _want_hip(grads):
         return _EXT.bulyan(grads, int(f), int(m))
     return reference.bulyan(grads, f, m)
+
+
+# ---------------------------------------------------------------------------- #
+# Optimizer ops (lists of tensors instead of the stacked matrix)
+
+from .adamw import (adamw8_plan, adamw8_state, adamw8_values,  # noqa: E402
+                    adamw_plan, adamw_step, grad_norm)

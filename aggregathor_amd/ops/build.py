@@ -26,8 +26,9 @@ OUT = OPS_DIR / "_gar_hip.so"
 OBJ = OPS_DIR / "_obj"
 
 SOURCES = [CSRC / "gar_ops.cpp", CSRC / "gar_kernels.hip",
-           CSRC / "bn_kernels.hip"]
-HEADERS = [CSRC / "gar_kernels.h"]
+           CSRC / "bn_kernels.hip", CSRC / "adamw_ops.cpp",
+           CSRC / "adamw_kernels.hip"]
+HEADERS = [CSRC / "gar_kernels.h", CSRC / "adamw_kernels.h"]
 
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 

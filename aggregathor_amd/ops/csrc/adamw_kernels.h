@@ -1,0 +1,101 @@
+// Launch API of the gfx950 optimizer kernels (implemented in
+// adamw_kernels.hip). Pure HIP host interface, like gar_kernels.h.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace adamw {
+
+// Element types of parameters and gradients.
+enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// Elements that share one scale in an 8-bit state.
+constexpr int kGroup = 32;
+// Elements that one workgroup updates.
+constexpr int kChunk = 4096;
+// Tensors of one update launch: their gradients' addresses travel in the
+// kernel's arguments, of which there are 4 KiB.
+constexpr int kMaxTensors = 448;
+// Spans of one norm launch, likewise, the workgroups of one such launch at
+// most, and the bytes that one of them reads at a time.
+constexpr int kMaxSpans = 160;
+constexpr int kNormBlocks = 2048;
+constexpr int kNormChunkBytes = 16384;
+
+// One parameter tensor of a plan. 32-bit states: m and r point to floats (r to
+// the mean square itself), ms and rs are null. 8-bit states: m and r point to
+// e4m3 codes (r to those of the mean square's root), ms and rs to their groups'
+// biased exponents.
+struct Tensor {
+  void* p;
+  void* m;
+  void* r;
+  uint8_t* ms;
+  uint8_t* rs;
+  long n;
+  uint32_t key;  // of the rounding's random bits
+  int type;      // of p
+};
+
+// Which part of which tensor a workgroup updates.
+struct Chunk {
+  int tensor;
+  int index;
+};
+
+// The gradients of a launch: null where a tensor has none, and two bits each
+// for their types.
+struct Grads {
+  const void* g[kMaxTensors];
+  uint32_t types[kMaxTensors / 16];
+};
+
+// A bit for each tensor of a launch that has a gradient.
+struct Present {
+  uint64_t bits[kMaxTensors / 64];
+};
+
+struct Hyper {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* norm;  // null: no clipping
+  double max_norm;
+};
+
+// Whether update() has a form for parameters of type p and gradients of type g.
+bool supported(int p, int g);
+
+// steps[i] += 1 and coefs[i] = {lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)} for
+// those of `count` tensors that are present.
+void begin_step(int* steps, float2* coefs, const Present& present, int count,
+                const Hyper& hyper, hipStream_t stream);
+
+// One AdamW step of the chunks [0, nchunks); grads.g[i] belongs to tensor
+// first + i of `tensors`, `steps` and `coefs`.
+void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
+            int first, const int* steps, const float2* coefs,
+            const Grads& grads, const Hyper& hyper, hipStream_t stream);
+
+// Spans of elements that lie back to back in memory: start[i] is the first
+// chunk (of kNormChunkBytes) of span i within the launch, start[count] their
+// number.
+struct Spans {
+  const void* ptr[kMaxSpans];
+  long n[kMaxSpans];
+  int start[kMaxSpans + 1];
+  int type[kMaxSpans];
+  int count;
+};
+
+// Workgroups, and so partial sums, of a launch over these spans.
+int norm_blocks(const Spans& spans);
+
+// partials[b] = the b-th workgroup's sum of squares.
+void norm_partials(const Spans& spans, double* partials, hipStream_t stream);
+
+// out = sqrt(sum of partials[0..count)).
+void norm_finish(const double* partials, int count, float* out,
+                 hipStream_t stream);
+
+}  // namespace adamw

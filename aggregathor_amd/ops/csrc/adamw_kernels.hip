@@ -1,0 +1,470 @@
+// gfx950 kernels of the optimizer step: the L2 norm over many tensors, and the
+// AdamW step over many tensors with states in 32 or in 8 bits.
+//
+// With g the gradient, scaled by s = min(1, max_norm / norm) where it is
+// clipped, and t the tensor's number of steps:
+//
+//   m = beta1 m + (1 - beta1) s g
+//   v = beta2 v + (1 - beta2) (s g)^2
+//   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+//
+// 8-bit states. Groups of 32 consecutive elements of a tensor share a power of
+// two (one byte, the exponent with its bias of 127), and each element of m and
+// of r = sqrt(v) is an e4m3 code times it. The root is kept rather than v since
+// its range in binades is half as wide. The power puts the group's largest
+// value into [128, 256], so that rounding up never leaves the format; 17
+// binades below it the format ends. A root that is not zero is never stored as
+// zero: it would make the next step divide by eps.
+// To nearest, an average that moves by 1 - beta2 = 0.1 % a step would stand
+// still in a format whose half step is 6 %. So codes are rounded up or down by
+// chance, without bias: floor(y / quantum + u), u from 16 bits of a hash of
+// (seed, tensor, step, element). The hash makes a step's result a function of
+// its inputs, the same on every rank and in every replay.
+// The step itself uses the new m and v before they are rounded.
+//
+// The arithmetic on m, v and their codes is plain IEEE fp32, one rounding an
+// operation (no contraction into fused multiply-adds), so that states can be
+// compared with another implementation's bit by bit.
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include "adamw_kernels.h"
+
+#pragma clang fp contract(off)
+
+namespace adamw {
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kQuads = kChunk / (4 * kBlock);  // quads of a thread
+
+// Four elements of T. Tensors start anywhere (a gradient is a view into the
+// flat gradient), so a quad is only aligned like its element: gfx950 loads and
+// stores it in one instruction all the same.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Quad {
+  T v[4];
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__hip_bfloat16 v) {
+  return __bfloat162float(v);
+}
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) {
+  return __float2bfloat16(v);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half(v);
+}
+
+// Loads elements [i, i + 4) below n; those behind it are zero.
+template <bool Full, typename T>
+__device__ __forceinline__ void load4(const T* base, long i, long n,
+                                      float (&out)[4]) {
+  if (Full || i + 4 <= n) {
+    Quad<T> q = *reinterpret_cast<const Quad<T>*>(base + i);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) out[c] = to_f32(q.v[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) out[c] = i + c < n ? to_f32(base[i + c]) : 0.f;
+  }
+}
+
+template <bool Full, typename T>
+__device__ __forceinline__ void store4(T* base, long i, long n,
+                                       const float (&x)[4]) {
+  if (Full || i + 4 <= n) {
+    Quad<T> q;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) q.v[c] = from_f32<T>(x[c]);
+    *reinterpret_cast<Quad<T>*>(base + i) = q;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (i + c < n) base[i + c] = from_f32<T>(x[c]);
+  }
+}
+
+// Four codes as one word, and back.
+struct __attribute__((packed, aligned(1))) Word {
+  uint32_t v;
+};
+
+template <bool Full>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* base, long i,
+                                               long n) {
+  if (Full || i + 4 <= n) return reinterpret_cast<const Word*>(base + i)->v;
+  uint32_t w = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (i + c < n) w |= (uint32_t)base[i + c] << (8 * c);
+  return w;
+}
+
+template <bool Full>
+__device__ __forceinline__ void store_codes(uint8_t* base, long i, long n,
+                                            uint32_t w) {
+  if (Full || i + 4 <= n) {
+    reinterpret_cast<Word*>(base + i)->v = w;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (i + c < n) base[i + c] = (uint8_t)(w >> (8 * c));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit states
+
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x9E3779B1u;
+  x ^= x >> 15;
+  x *= 0x85EBCA77u;
+  return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ void decode(uint32_t w, float scale,
+                                       float (&out)[4]) {
+  auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  out[0] = lo[0] * scale;
+  out[1] = lo[1] * scale;
+  out[2] = hi[0] * scale;
+  out[3] = hi[1] * scale;
+}
+
+__device__ __forceinline__ uint32_t encode(const float (&z)[4]) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], w, true);
+}
+
+// Power of two with this biased exponent.
+__device__ __forceinline__ float pow2(uint32_t biased) {
+  return __uint_as_float(biased << 23);
+}
+
+// x times inv (a power of two, 1 / the group's scale), rounded to a value that
+// e4m3 has: up with the probability of chance / 2^16. What is not finite
+// becomes a NaN, since the format has no infinity.
+__device__ __forceinline__ float round_by_chance(float x, float inv,
+                                                 uint32_t chance, float least) {
+  const float y = fabsf(x) * inv;
+  uint32_t e = __float_as_uint(y) >> 23;
+  e = e < 121 ? 121 : e;  // below 2^-6 the quantum stays 2^-9
+  float t = floorf(y * pow2(257 - e) + (float)chance * 0x1p-16f);
+  if (y > 0.f) t = fmaxf(t, least);
+  const float z = copysignf(t * pow2(e - 3), x);
+  return y < INFINITY ? z : NAN;
+}
+
+// Largest of a value over the eight lanes that share a group.
+__device__ __forceinline__ uint32_t max8(uint32_t v) {
+  // xor 1, xor 2 within four lanes, then each four against the other.
+  uint32_t o = __builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);
+  v = v > o ? v : o;
+  o = __builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);
+  v = v > o ? v : o;
+  o = __builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true);
+  return v > o ? v : o;
+}
+
+// Bits of the largest |x| that is finite; as whole numbers they order alike.
+__device__ __forceinline__ uint32_t top_bits(const float (&x)[4]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t b = __float_as_uint(x[c]) & 0x7FFFFFFFu;
+    b = b < 0x7F800000u ? b : 0u;
+    top = top > b ? top : b;
+  }
+  return top;
+}
+
+// ---------------------------------------------------------------------------
+// The update
+
+// What all elements of a workgroup share.
+struct Common {
+  float clip, beta1, rest1, beta2, rest2, eps, keep, rate, unbias;
+  uint32_t key;
+};
+
+__device__ __forceinline__ void moments(const Common& k, const float (&g)[4],
+                                        float (&m)[4], float (&v)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const float s = g[c] * k.clip;
+    m[c] = m[c] * k.beta1 + s * k.rest1;
+    v[c] = v[c] * k.beta2 + s * s * k.rest2;
+  }
+}
+
+__device__ __forceinline__ void move(const Common& k, const float (&m)[4],
+                                     const float (&root)[4], float (&p)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    p[c] = p[c] * k.keep - k.rate * (m[c] / (root[c] * k.unbias + k.eps));
+}
+
+template <int Bits, typename P, typename G, bool Full>
+__device__ __forceinline__ void update_chunk(const Tensor& t, const G* grad,
+                                             long start, const Common& k) {
+  P* const param = reinterpret_cast<P*>(t.p);
+  const long n = t.n;
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    const long i = start + 4 * ((long)q * kBlock + threadIdx.x);
+    float p[4], g[4], m[4], v[4], root[4];
+    load4<Full>(param, i, n, p);
+    load4<Full>(grad, i, n, g);
+    if constexpr (Bits == 32) {
+      float* const mp = reinterpret_cast<float*>(t.m);
+      float* const vp = reinterpret_cast<float*>(t.r);
+      load4<Full>(mp, i, n, m);
+      load4<Full>(vp, i, n, v);
+      moments(k, g, m, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
+      store4<Full>(mp, i, n, m);
+      store4<Full>(vp, i, n, v);
+    } else {
+      uint8_t* const mc = reinterpret_cast<uint8_t*>(t.m);
+      uint8_t* const rc = reinterpret_cast<uint8_t*>(t.r);
+      const long group = i / kGroup;
+      const bool some = Full || i < n;
+      decode(load_codes<Full>(mc, i, n), some ? pow2(t.ms[group]) : 0.f, m);
+      decode(load_codes<Full>(rc, i, n), some ? pow2(t.rs[group]) : 0.f, root);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = root[c] * root[c];
+      moments(k, g, m, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
+
+      // All eight lanes of a group come here, also those behind the end.
+      const uint32_t em = max8(top_bits(m)) >> 23;
+      const uint32_t ev = max8(top_bits(v)) >> 23;
+      const uint32_t sm = em < 14 ? 7 : em - 7;
+      const uint32_t sr = (uint32_t)(((int)ev - 127) >> 1) + 120;
+      const float im = pow2(254 - sm), ir = pow2(254 - sr);
+      float zm[4], zr[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t h = mix((uint32_t)(i + c) ^ (k.key + 0x9E3779B9u * (uint32_t)(i >> 32)));
+        zm[c] = round_by_chance(m[c], im, h & 0xFFFFu, 0.f);
+        zr[c] = round_by_chance(root[c], ir, h >> 16, 1.f);
+      }
+      store_codes<Full>(mc, i, n, encode(zm));
+      store_codes<Full>(rc, i, n, encode(zr));
+      if (some && threadIdx.x % (kGroup / 4) == 0) {
+        t.ms[group] = (uint8_t)sm;
+        t.rs[group] = (uint8_t)sr;
+      }
+    }
+    move(k, m, root, p);
+    store4<Full>(param, i, n, p);
+  }
+}
+
+template <int Bits, typename P, typename G>
+__device__ __forceinline__ void update_tensor(const Tensor& t, const void* grad,
+                                              long start, const Common& k) {
+  const G* const g = reinterpret_cast<const G*>(grad);
+  if (start + kChunk <= t.n)
+    update_chunk<Bits, P, G, true>(t, g, start, k);
+  else
+    update_chunk<Bits, P, G, false>(t, g, start, k);
+}
+
+struct Scalars {
+  float beta1, rest1, beta2, rest2, eps, keep, max_norm;
+  const float* norm;
+};
+
+template <int Bits>
+__global__ __launch_bounds__(kBlock) void update_kernel(
+    const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
+    int first, const int* __restrict__ steps,
+    const float2* __restrict__ coefs, const Grads grads, const Scalars s) {
+  const Chunk chunk = chunks[blockIdx.x];
+  const int at = chunk.tensor - first;
+  const void* const grad = grads.g[at];
+  if (grad == nullptr) return;
+  const Tensor t = tensors[chunk.tensor];
+  const float2 coef = coefs[chunk.tensor];
+  Common k;
+  k.clip = 1.f;
+  if (s.norm != nullptr) {
+    const float norm = *s.norm;
+    k.clip = norm <= s.max_norm ? 1.f : s.max_norm / norm;
+  }
+  k.beta1 = s.beta1;
+  k.rest1 = s.rest1;
+  k.beta2 = s.beta2;
+  k.rest2 = s.rest2;
+  k.eps = s.eps;
+  k.keep = s.keep;
+  k.rate = coef.x;
+  k.unbias = coef.y;
+  k.key = Bits == 8 ? mix(t.key + (uint32_t)steps[chunk.tensor]) : 0;
+  const long start = (long)chunk.index * kChunk;
+  const uint32_t gt = (grads.types[at / 16] >> (2 * (at % 16))) & 3;
+  switch (t.type * 4 + gt) {
+    case kF32 * 4 + kF32:
+      return update_tensor<Bits, float, float>(t, grad, start, k);
+    case kF32 * 4 + kBF16:
+      return update_tensor<Bits, float, __hip_bfloat16>(t, grad, start, k);
+    case kF32 * 4 + kF16:
+      return update_tensor<Bits, float, __half>(t, grad, start, k);
+    case kBF16 * 4 + kBF16:
+      return update_tensor<Bits, __hip_bfloat16, __hip_bfloat16>(t, grad, start,
+                                                                 k);
+    case kF16 * 4 + kF16:
+      return update_tensor<Bits, __half, __half>(t, grad, start, k);
+  }
+}
+
+__global__ __launch_bounds__(kMaxTensors) void begin_step_kernel(
+    int* steps, float2* coefs, Present present, int count, double lr,
+    double beta1, double beta2) {
+  const int i = threadIdx.x;
+  if (i >= count || !(present.bits[i / 64] >> (i % 64) & 1)) return;
+  const int t = steps[i] + 1;
+  steps[i] = t;
+  // In 64 bits: 1 - beta^t loses what 32 hold when it is near zero.
+  coefs[i] = make_float2((float)(lr / (1.0 - pow(beta1, (double)t))),
+                         (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))));
+}
+
+// ---------------------------------------------------------------------------
+// The norm. Squares are summed in 64 bits: no sum of them is too long, none of
+// fp32 overflows or vanishes, and the vector units have the rate for it at
+// four bytes an element. Which workgroup adds which elements is fixed by the
+// spans alone, so the result is the same every time.
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const T* base, long begin,
+                                                long n) {
+  constexpr int kElems = kNormChunkBytes / sizeof(T);
+  double sum[4] = {0, 0, 0, 0};
+  if (begin + kElems <= n) {
+#pragma unroll
+    for (int q = 0; q < kElems / (4 * kBlock); ++q) {
+      float x[4];
+      load4<true>(base, begin + 4 * ((long)q * kBlock + threadIdx.x), n, x);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = fma((double)x[c], (double)x[c], sum[c]);
+    }
+  } else {
+    for (long i = begin + 4 * threadIdx.x; i < n; i += 4 * kBlock) {
+      float x[4];
+      load4<false>(base, i, n, x);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = fma((double)x[c], (double)x[c], sum[c]);
+    }
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// Sum over the workgroup, in thread 0.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[kBlock / 64];
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
+  __syncthreads();
+  v = 0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < kBlock / 64; ++w) v += part[w];
+  return v;
+}
+
+__global__ __launch_bounds__(kBlock) void norm_kernel(const Spans spans,
+                                                      double* partials) {
+  double sum = 0;
+  int span = 0;
+  for (int c = blockIdx.x; c < spans.start[spans.count]; c += gridDim.x) {
+    while (c >= spans.start[span + 1]) ++span;
+    const long bytes = (long)(c - spans.start[span]) * kNormChunkBytes;
+    const void* const ptr = spans.ptr[span];
+    const long n = spans.n[span];
+    switch (spans.type[span]) {
+      case kF32:
+        sum += chunk_squares((const float*)ptr, bytes / 4, n);
+        break;
+      case kBF16:
+        sum += chunk_squares((const __hip_bfloat16*)ptr, bytes / 2, n);
+        break;
+      case kF16:
+        sum += chunk_squares((const __half*)ptr, bytes / 2, n);
+        break;
+    }
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(kBlock) void norm_finish_kernel(
+    const double* __restrict__ partials, int count, float* out) {
+  double sum = 0;
+  for (int i = threadIdx.x; i < count; i += kBlock) sum += partials[i];
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) *out = (float)sqrt(sum);
+}
+
+}  // namespace
+
+bool supported(int p, int g) { return p == g || p == kF32; }
+
+void begin_step(int* steps, float2* coefs, const Present& present, int count,
+                const Hyper& h, hipStream_t stream) {
+  begin_step_kernel<<<1, kMaxTensors, 0, stream>>>(steps, coefs, present, count,
+                                                   h.lr, h.beta1, h.beta2);
+}
+
+void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
+            int first, const int* steps, const float2* coefs,
+            const Grads& grads, const Hyper& h, hipStream_t stream) {
+  const Scalars s = {(float)h.beta1,
+                     (float)(1.0 - h.beta1),
+                     (float)h.beta2,
+                     (float)(1.0 - h.beta2),
+                     (float)h.eps,
+                     (float)(1.0 - h.lr * h.weight_decay),
+                     (float)h.max_norm,
+                     h.norm};
+  if (bits == 8)
+    update_kernel<8><<<dim3((unsigned)nchunks), kBlock, 0, stream>>>(
+        tensors, chunks, first, steps, coefs, grads, s);
+  else
+    update_kernel<32><<<dim3((unsigned)nchunks), kBlock, 0, stream>>>(
+        tensors, chunks, first, steps, coefs, grads, s);
+}
+
+int norm_blocks(const Spans& spans) {
+  const int chunks = spans.start[spans.count];
+  return chunks < kNormBlocks ? chunks : kNormBlocks;
+}
+
+void norm_partials(const Spans& spans, double* partials, hipStream_t stream) {
+  norm_kernel<<<norm_blocks(spans), kBlock, 0, stream>>>(spans, partials);
+}
+
+void norm_finish(const double* partials, int count, float* out,
+                 hipStream_t stream) {
+  norm_finish_kernel<<<1, kBlock, 0, stream>>>(partials, count, out);
+}
+
+}  // namespace adamw

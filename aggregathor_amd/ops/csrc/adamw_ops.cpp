@@ -1,0 +1,441 @@
+// Torch glue for the optimizer kernels (adamw_kernels.hip): the plan that an
+// optimizer keeps for its tensors, its step, and the norm over many tensors.
+// Like the GAR ops, all launches go to the current HIP stream of the tensors'
+// device, nothing waits for the device, and everything can be captured into a
+// graph.
+
+#include <torch/extension.h>
+
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPStream.h>
+
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <optional>
+#include <vector>
+
+#include "adamw_kernels.h"
+
+namespace {
+
+using torch::Tensor;
+
+int dtype_of(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32:
+      return adamw::kF32;
+    case torch::kBFloat16:
+      return adamw::kBF16;
+    case torch::kFloat16:
+      return adamw::kF16;
+    default:
+      TORCH_CHECK(false, what, ": expected fp32, bf16 or fp16, got ",
+                  t.scalar_type());
+  }
+}
+
+// Bytes [lo, hi) that a tensor's elements lie in.
+struct Range {
+  uintptr_t lo, hi;
+};
+
+Range range_of(const Tensor& t) {
+  const auto lo = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {lo, lo};
+  uintptr_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    last += (uintptr_t)(t.size(d) - 1) * t.stride(d);
+  return {lo, lo + (last + 1) * t.element_size()};
+}
+
+// Whether equal places in memory hold equal elements of both.
+bool same_layout(const Tensor& a, const Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  if (a.numel() < 2) return true;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
+uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x9E3779B1u;
+  x ^= x >> 15;
+  x *= 0x85EBCA77u;
+  return x ^ (x >> 16);
+}
+
+bool capturing() {
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() !=
+         c10::hip::CaptureStatus::None;
+}
+
+// Tables that a captured graph reads stay for the process's life: a replay
+// after the plan is gone would take addresses from memory that is something
+// else by then. A few KiB each. Never destroyed.
+std::vector<Tensor>& captured_tables() {
+  static auto* kept = new std::vector<Tensor>();
+  return *kept;
+}
+
+template <typename T>
+Tensor upload(const std::vector<T>& host, const c10::Device& device) {
+  auto bytes = torch::from_blob(const_cast<T*>(host.data()),
+                                {(int64_t)(host.size() * sizeof(T))},
+                                torch::kUInt8);
+  return bytes.to(device);  // waits until `host` has been read
+}
+
+class Plan {
+ public:
+  Plan(int bits, std::vector<Tensor> params, std::vector<Tensor> m,
+       std::vector<Tensor> ms, std::vector<Tensor> r, std::vector<Tensor> rs,
+       Tensor steps, int64_t seed)
+      : bits_(bits),
+        params_(std::move(params)),
+        m_(std::move(m)),
+        ms_(std::move(ms)),
+        r_(std::move(r)),
+        rs_(std::move(rs)),
+        steps_(std::move(steps)),
+        seed_((uint32_t)seed) {
+    TORCH_CHECK(!params_.empty(), "adamw: a plan needs a parameter");
+    lay_out();
+  }
+
+  void step(const std::vector<std::optional<Tensor>>& grads, double lr,
+            double beta1, double beta2, double eps, double weight_decay,
+            const std::optional<Tensor>& norm, double max_norm) {
+    const size_t count = params_.size();
+    TORCH_CHECK(grads.size() == count, "adamw: ", count, " parameters, but ",
+                grads.size(), " gradients");
+    const c10::Device device = params_[0].device();
+    c10::DeviceGuard guard(device);
+    if (stale()) lay_out();
+
+    adamw::Hyper hyper{lr, beta1, beta2, eps, weight_decay, nullptr, max_norm};
+    if (norm) {
+      TORCH_CHECK(norm->device() == device && norm->numel() == 1 &&
+                      norm->scalar_type() == torch::kFloat32,
+                  "adamw: norm is one fp32 number on the parameters' device");
+      check_apart(*norm, "adamw: norm");
+      hyper.norm = norm->data_ptr<float>();
+    }
+    // Everything is checked before anything is launched.
+    std::vector<Tensor> held(count);
+    std::vector<int> types(count, 0);
+    for (size_t i = 0; i < count; ++i) {
+      if (!grads[i]) continue;
+      const Tensor& g = *grads[i];
+      const Tensor& p = params_[i];
+      TORCH_CHECK(g.layout() == torch::kStrided,
+                  "adamw: gradient ", i, " is not dense");
+      TORCH_CHECK(g.device() == device, "adamw: gradient ", i, " is on ",
+                  g.device(), ", its parameter on ", device);
+      TORCH_CHECK(g.sizes() == p.sizes(), "adamw: gradient ", i,
+                  " has the shape ", g.sizes(), ", its parameter ", p.sizes());
+      types[i] = dtype_of(g, "adamw: gradient");
+      TORCH_CHECK(adamw::supported(table_[i].type, types[i]),
+                  "adamw: gradient ", i, " is ", g.scalar_type(),
+                  ", its parameter ", p.scalar_type(),
+                  " (the same type, or fp32 parameters)");
+      check_apart(g, "adamw: gradient");
+      held[i] = g.resolve_neg();
+    }
+    for (size_t i = 0; i < count; ++i) {
+      if (!held[i].defined() || same_layout(held[i], params_[i])) continue;
+      auto moved = torch::empty_strided(params_[i].sizes(),
+                                        params_[i].strides(),
+                                        held[i].options());
+      held[i] = moved.copy_(held[i]);
+    }
+
+    const auto current = c10::hip::getCurrentHIPStream();
+    const auto stream = current.stream();
+    if (capturing()) {
+      if (!captured_)
+        for (const Tensor& t : {device_table_, device_chunks_, coefs_})
+          captured_tables().push_back(t);
+      captured_ = true;
+    } else if (current != laid_out_on_) {
+      // The allocator must not give these to others before this step is done.
+      for (const Tensor& t : {device_table_, device_chunks_, coefs_})
+        t.record_stream(
+            c10::hip::HIPStreamMasqueradingAsCUDA(current).unwrap());
+    }
+    const auto* tensors =
+        reinterpret_cast<const adamw::Tensor*>(device_table_.data_ptr());
+    const auto* chunks =
+        reinterpret_cast<const adamw::Chunk*>(device_chunks_.data_ptr());
+    auto* coefs = reinterpret_cast<float2*>(coefs_.data_ptr());
+    int* steps = steps_.data_ptr<int>();
+    for (size_t first = 0; first < count; first += adamw::kMaxTensors) {
+      const size_t last = std::min(count, first + adamw::kMaxTensors);
+      adamw::Grads g{};
+      adamw::Present present{};
+      bool any = false;
+      for (size_t i = first; i < last; ++i) {
+        if (!held[i].defined()) continue;
+        const size_t k = i - first;
+        any = true;
+        g.g[k] = held[i].data_ptr();
+        g.types[k / 16] |= (uint32_t)types[i] << (2 * (k % 16));
+        present.bits[k / 64] |= 1ull << (k % 64);
+      }
+      if (!any) continue;
+      adamw::begin_step(steps + first, coefs + first, present,
+                        (int)(last - first), hyper, stream);
+      C10_HIP_CHECK(hipGetLastError());
+      const int64_t begin = chunk_start_[first];
+      const int64_t nchunks = chunk_start_[last] - begin;
+      if (nchunks > 0) {
+        adamw::update(bits_, tensors, chunks + begin, nchunks, (int)first,
+                      steps, coefs, g, hyper, stream);
+        C10_HIP_CHECK(hipGetLastError());
+      }
+    }
+    // What autograd has saved of the parameters is out of date.
+    for (size_t i = 0; i < count; ++i)
+      if (held[i].defined() && !params_[i].is_inference())
+        params_[i].unsafeGetTensorImpl()->bump_version();
+  }
+
+ private:
+  // Whether a tensor of the plan has got other memory since it was laid out
+  // (`param.data = ...`, or a module moved).
+  bool stale() const {
+    if (steps_.data_ptr() != steps_at_ ||
+        steps_.numel() != (int64_t)params_.size())
+      return true;
+    for (size_t i = 0; i < params_.size(); ++i) {
+      const auto& t = table_[i];
+      if (params_[i].data_ptr() != t.p || m_[i].data_ptr() != t.m ||
+          r_[i].data_ptr() != t.r || params_[i].numel() != t.n ||
+          params_[i].device() != steps_.device() ||
+          dtype_of(params_[i], "adamw: parameter") != t.type ||
+          !same_layout(params_[i], m_[i]) || !same_layout(params_[i], r_[i]))
+        return true;
+      if (bits_ == 8 &&
+          (ms_[i].data_ptr() != t.ms || rs_[i].data_ptr() != t.rs ||
+           ms_[i].numel() != rs_[i].numel() ||
+           ms_[i].numel() != (t.n + adamw::kGroup - 1) / adamw::kGroup))
+        return true;
+    }
+    return false;
+  }
+
+  void check_state(const Tensor& s, const Tensor& p, torch::ScalarType type,
+                   const char* what, size_t i) {
+    TORCH_CHECK(s.scalar_type() == type, "adamw: ", what, " ", i, " is ",
+                s.scalar_type(), ", expected ", type);
+    TORCH_CHECK(s.device() == p.device(), "adamw: ", what, " ", i, " is on ",
+                s.device(), ", its parameter on ", p.device());
+    TORCH_CHECK(same_layout(s, p), "adamw: ", what, " ", i,
+                " has another shape or other strides than its parameter");
+  }
+
+  void lay_out() {
+    TORCH_CHECK(!capturing(),
+                "adamw: a plan cannot be laid out while a graph is captured "
+                "(a parameter or state has other memory than before: run a "
+                "step before the capture)");
+    const size_t count = params_.size();
+    const c10::Device device = params_[0].device();
+    TORCH_CHECK(m_.size() == count && r_.size() == count &&
+                    (bits_ == 32 || (ms_.size() == count && rs_.size() == count)),
+                "adamw: as many states as parameters are needed");
+    TORCH_CHECK(steps_.device() == device && steps_.dim() == 1 &&
+                    steps_.size(0) == (int64_t)count &&
+                    steps_.is_contiguous() &&
+                    steps_.scalar_type() == torch::kInt32,
+                "adamw: steps is a contiguous int32 tensor of one count for "
+                "each parameter, on their device");
+    const auto state_type =
+        bits_ == 8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
+    std::vector<adamw::Tensor> table(count);
+    std::vector<adamw::Chunk> chunks;
+    std::vector<int64_t> chunk_start(count + 1, 0);
+    std::vector<Range> written{range_of(steps_)};
+    for (size_t i = 0; i < count; ++i) {
+      const Tensor& p = params_[i];
+      TORCH_CHECK(p.is_cuda() && p.layout() == torch::kStrided,
+                  "adamw: expected dense GPU parameters");
+      TORCH_CHECK(p.device() == device,
+                  "adamw: the parameters of a plan are on one device");
+      TORCH_CHECK(p.is_non_overlapping_and_dense(), "adamw: parameter ", i,
+                  " of shape ", p.sizes(), " and strides ", p.strides(),
+                  " does not fill its memory");
+      check_state(m_[i], p, state_type, "exp_avg", i);
+      check_state(r_[i], p, state_type,
+                  bits_ == 8 ? "exp_avg_root" : "exp_avg_sq", i);
+      const int64_t n = p.numel();
+      auto& t = table[i];
+      t.p = p.data_ptr();
+      t.m = m_[i].data_ptr();
+      t.r = r_[i].data_ptr();
+      t.n = n;
+      t.key = mix(seed_ + 0x9E3779B9u * (uint32_t)(i + 1));
+      t.type = dtype_of(p, "adamw: parameter");
+      written.push_back(range_of(p));
+      written.push_back(range_of(m_[i]));
+      written.push_back(range_of(r_[i]));
+      if (bits_ == 8) {
+        const int64_t groups = (n + adamw::kGroup - 1) / adamw::kGroup;
+        for (const Tensor* s : {&ms_[i], &rs_[i]}) {
+          TORCH_CHECK(s->scalar_type() == torch::kFloat8_e8m0fnu &&
+                          s->device() == device && s->dim() == 1 &&
+                          s->size(0) == groups && s->is_contiguous(),
+                      "adamw: the scales of state ", i,
+                      " are a contiguous e8m0 tensor of ", groups,
+                      " elements on its parameter's device");
+          written.push_back(range_of(*s));
+        }
+        t.ms = reinterpret_cast<uint8_t*>(ms_[i].data_ptr());
+        t.rs = reinterpret_cast<uint8_t*>(rs_[i].data_ptr());
+      }
+      const int64_t parts = (n + adamw::kChunk - 1) / adamw::kChunk;
+      TORCH_CHECK(parts <= INT32_MAX, "adamw: parameter ", i, " is too large");
+      for (int64_t c = 0; c < parts; ++c)
+        chunks.push_back({(int)i, (int)c});
+      chunk_start[i + 1] = chunk_start[i] + parts;
+    }
+    std::sort(written.begin(), written.end(),
+              [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    written.erase(std::remove_if(written.begin(), written.end(),
+                                 [](const Range& r) { return r.lo == r.hi; }),
+                  written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      TORCH_CHECK(written[i - 1].hi <= written[i].lo,
+                  "adamw: parameters, states and steps share memory");
+    c10::DeviceGuard guard(device);
+    device_table_ = upload(table, device);
+    if (chunks.empty()) chunks.push_back({0, 0});
+    device_chunks_ = upload(chunks, device);
+    coefs_ = torch::empty({(int64_t)count, 2},
+                          torch::TensorOptions().device(device).dtype(
+                              torch::kFloat32));
+    laid_out_on_ = c10::hip::getCurrentHIPStream();
+    steps_at_ = steps_.data_ptr();
+    table_ = std::move(table);
+    chunk_start_ = std::move(chunk_start);
+    written_ = std::move(written);
+    captured_ = false;
+  }
+
+  // What the step reads must not be what it writes.
+  void check_apart(const Tensor& t, const char* what) const {
+    const Range r = range_of(t);
+    if (r.lo == r.hi) return;
+    auto it = std::upper_bound(
+        written_.begin(), written_.end(), r.lo,
+        [](uintptr_t v, const Range& w) { return v < w.hi; });
+    TORCH_CHECK(it == written_.end() || it->lo >= r.hi, what,
+                " shares memory with a parameter or state");
+  }
+
+  int bits_;
+  std::vector<Tensor> params_, m_, ms_, r_, rs_;
+  Tensor steps_;
+  uint32_t seed_;
+  std::vector<adamw::Tensor> table_;
+  std::vector<int64_t> chunk_start_;
+  std::vector<Range> written_;
+  Tensor device_table_, device_chunks_, coefs_;
+  c10::hip::HIPStream laid_out_on_ = c10::hip::getDefaultHIPStream();
+  const void* steps_at_ = nullptr;
+  bool captured_ = false;
+};
+
+Tensor grad_norm(const std::vector<Tensor>& tensors) {
+  TORCH_CHECK(!tensors.empty(), "grad_norm: expected a tensor");
+  const c10::Device device = tensors[0].device();
+  TORCH_CHECK(tensors[0].is_cuda(), "grad_norm: expected GPU tensors");
+  c10::DeviceGuard guard(device);
+  const auto stream = c10::hip::getCurrentHIPStream().stream();
+
+  std::vector<std::unique_ptr<adamw::Spans>> launches;
+  std::vector<Tensor> held;
+  const char* end = nullptr;  // of the last span
+  for (const Tensor& given : tensors) {
+    TORCH_CHECK(given.layout() == torch::kStrided && given.device() == device,
+                "grad_norm: expected dense tensors on one device");
+    const int type = dtype_of(given, "grad_norm");
+    int64_t n = given.numel();
+    if (n == 0) continue;
+    // The order of the elements does not matter, only that there are no gaps.
+    Tensor t = given;
+    if (!t.is_non_overlapping_and_dense()) {
+      t = t.contiguous();
+      held.push_back(t);
+    }
+    const char* ptr = (const char*)t.data_ptr();
+    if (!launches.empty()) {
+      auto& s = *launches.back();
+      const int last = s.count - 1;
+      // Tensors that lie back to back, as views into a flat gradient do, are
+      // one span: fewer partly filled chunks, and hardly any search.
+      if (ptr == end && type == s.type[last]) {
+        const int64_t all = s.n[last] + n;
+        const int64_t chunks = (all * t.element_size() +
+                                adamw::kNormChunkBytes - 1) /
+                               adamw::kNormChunkBytes;
+        TORCH_CHECK(s.start[last] + chunks <= INT32_MAX,
+                    "grad_norm: too many elements");
+        s.n[last] = all;
+        s.start[last + 1] = (int)(s.start[last] + chunks);
+        end = ptr + n * t.element_size();
+        continue;
+      }
+    }
+    if (launches.empty() || launches.back()->count == adamw::kMaxSpans) {
+      launches.push_back(std::make_unique<adamw::Spans>());
+      launches.back()->count = 0;
+      launches.back()->start[0] = 0;
+    }
+    auto& s = *launches.back();
+    const int i = s.count++;
+    const int64_t chunks =
+        (n * t.element_size() + adamw::kNormChunkBytes - 1) /
+        adamw::kNormChunkBytes;
+    TORCH_CHECK(s.start[i] + chunks <= INT32_MAX,
+                "grad_norm: too many elements");
+    s.ptr[i] = ptr;
+    s.n[i] = n;
+    s.type[i] = type;
+    s.start[i + 1] = (int)(s.start[i] + chunks);
+    end = ptr + n * t.element_size();
+  }
+  auto options = torch::TensorOptions().device(device);
+  auto out = torch::empty({}, options.dtype(torch::kFloat32));
+  int count = 0;
+  for (auto& s : launches) count += adamw::norm_blocks(*s);
+  auto partials =
+      torch::empty({std::max(count, 1)}, options.dtype(torch::kFloat64));
+  double* at = partials.data_ptr<double>();
+  for (auto& s : launches) {
+    adamw::norm_partials(*s, at, stream);
+    C10_HIP_CHECK(hipGetLastError());
+    at += adamw::norm_blocks(*s);
+  }
+  adamw::norm_finish(partials.data_ptr<double>(), count, out.data_ptr<float>(),
+                     stream);
+  C10_HIP_CHECK(hipGetLastError());
+  return out;
+}
+
+}  // namespace
+
+void register_adamw(pybind11::module& mod) {
+  namespace py = pybind11;
+  py::class_<Plan>(mod, "AdamWPlan")
+      .def(py::init<int, std::vector<Tensor>, std::vector<Tensor>,
+                    std::vector<Tensor>, std::vector<Tensor>,
+                    std::vector<Tensor>, Tensor, int64_t>())
+      .def("step", &Plan::step);
+  mod.def("grad_norm", &grad_norm,
+          "L2 norm over all elements of many tensors (gfx950)");
+}

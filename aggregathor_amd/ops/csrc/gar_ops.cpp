@@ -192,7 +192,10 @@ std::vector<torch::Tensor> bn_bwd_train(torch::Tensor dy, torch::Tensor x,
   return {dx, dweight, dbias};
 }
 
+void register_adamw(pybind11::module& mod);  // adamw_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
+  register_adamw(mod);
   mod.def("bn_fwd_train", &bn_fwd_train,
           "Fused NHWC BatchNorm training forward (gfx950)");
   mod.def("bn_bwd_train", &bn_bwd_train,

@@ -1,0 +1,202 @@
+"""AdamW over the framework's optimizer kernels (:mod:`aggregathor_amd.ops`).
+
+One launch updates every parameter of a group, whatever their number; step
+counts, clipping and the rounding's random bits live on the device, so a step
+waits for nothing and can be captured into a graph (a captured
+``torch.optim.Adam`` needs ``capturable=True`` for that). States take 8 bytes an
+element, or 2.06 with ``state_bits=8``.
+
+The result is a function of parameters, gradients and states alone, bit by bit:
+ranks that hold the same aggregated gradient keep the same parameters.
+"""
+
+import torch
+
+from . import ops, tools
+from .ops import adamw_reference as reference
+
+_STATES = {32: ("exp_avg", "exp_avg_sq"),
+           8: ("exp_avg", "exp_avg_scale", "exp_avg_root",
+               "exp_avg_root_scale")}
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (Adam with decoupled weight decay).
+
+    Args:
+      params:        parameters or parameter groups
+      lr, betas, eps, weight_decay: as in ``torch.optim.AdamW`` (per group)
+      state_bits:    32 or 8, the width of the states (per group)
+      max_norm:      clip the gradient of all groups together to this L2 norm
+                     (None: no clipping; parameters on one device only)
+      rounding_seed: of the 8-bit states' rounding
+
+    A parameter without a gradient is left out of the step, its step count too.
+    Each parameter's ``state`` holds ``step`` and the state tensors; they may be
+    changed in place, and replaced by :meth:`load_state_dict`, which also takes
+    the state of a ``torch.optim.Adam`` or ``AdamW`` (32 bits).
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+                 weight_decay=1e-2, state_bits=32, max_norm=None,
+                 rounding_seed=0):
+        if max_norm is not None and not max_norm > 0:
+            raise tools.UserException(
+                f"adamw: expected a positive norm to clip to, got {max_norm}")
+        self.max_norm = max_norm
+        self.rounding_seed = rounding_seed
+        self._plans = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps,
+                                      weight_decay=weight_decay,
+                                      state_bits=state_bits))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        self._check_bits(self.param_groups[-1])
+        self._plans = None
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = None
+
+    def __getstate__(self):
+        # Plans are laid out anew where the optimizer is copied to.
+        return dict(super().__getstate__(), max_norm=self.max_norm,
+                    rounding_seed=self.rounding_seed)
+
+    @staticmethod
+    def _check_bits(group):
+        if group["state_bits"] not in _STATES:
+            raise tools.UserException("adamw: states have 32 or 8 bits, not "
+                                      f"{group['state_bits']!r}")
+
+    # ------------------------------------------------------------------ #
+
+    def _lay_out(self):
+        """Make the states that are missing, and a plan for each group (and
+        each device of its parameters)."""
+        self._plans, self._first_steps = [], []
+        for index, group in enumerate(self.param_groups):
+            self._check_bits(group)
+            bits = group["state_bits"]
+            by_device = {}
+            for p in group["params"]:
+                by_device.setdefault(p.device, []).append(p)
+            for device, params in by_device.items():
+                steps = torch.zeros(len(params), dtype=torch.int32,
+                                    device=device)
+                columns = [[] for _ in _STATES[bits]]
+                for i, p in enumerate(params):
+                    state = self.state[p]
+                    if "step" in state:
+                        steps[i] = state["step"]
+                    else:
+                        fresh = (ops.adamw8_state(p) if bits == 8 else
+                                 [torch.zeros_like(p, dtype=torch.float32,
+                                                   requires_grad=False)
+                                  for _ in range(2)])
+                        state.update(zip(_STATES[bits], fresh))
+                    state["step"] = steps[i]  # a view: the plan counts there
+                    for column, name in zip(columns, _STATES[bits]):
+                        column.append(state[name])
+                if bits == 8:
+                    plan = ops.adamw8_plan(params, *columns, steps,
+                                           seed=self.rounding_seed + index)
+                else:
+                    plan = ops.adamw_plan(params, *columns, steps)
+                self._plans.append((group, params, plan))
+                self._first_steps.append(self.state[params[0]]["step"])
+
+    def _state_kept(self):
+        """Whether the plans still hold the state (a user may have cleared it;
+        the first parameter of each tells)."""
+        return all(self.state[params[0]].get("step") is first
+                   for (_, params, _), first in zip(self._plans,
+                                                    self._first_steps))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step over all parameters that have a gradient."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if self._plans is None or not self._state_kept():
+            self._lay_out()
+        grads = [[p.grad for p in params] for _, params, _ in self._plans]
+        norm = None
+        if self.max_norm is not None:
+            present = [g for part in grads for g in part if g is not None]
+            if not present:
+                return loss
+            norm = ops.grad_norm(present)
+        for (group, _, plan), part in zip(self._plans, grads):
+            beta1, beta2 = group["betas"]
+            ops.adamw_step(plan, part, lr=float(group["lr"]), beta1=beta1,
+                           beta2=beta2, eps=group["eps"],
+                           weight_decay=group["weight_decay"], norm=norm,
+                           max_norm=self.max_norm)
+        return loss
+
+    # ------------------------------------------------------------------ #
+
+    def load_state_dict(self, state_dict):
+        """Load what :meth:`state_dict` gave. (The base class would cast every
+        state to its parameter's type.)"""
+        groups = []
+        for group in state_dict["param_groups"]:
+            group = dict(group)
+            group.setdefault("state_bits", 32)
+            self._check_bits(group)
+            groups.append(group)
+        saved = [i for group in groups for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        bits = [group["state_bits"] for group in groups
+                for _ in group["params"]]
+        if len(saved) != len(params):
+            raise ValueError("loaded state dict has another number of "
+                             "parameters than the optimizer")
+        states = {p: self._loaded(state_dict["state"][i], p, b)
+                  for i, p, b in zip(saved, params, bits)
+                  if i in state_dict["state"]}
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self.state.update(states)
+        self._plans = None
+
+    @staticmethod
+    def _loaded(state, p, bits):
+        missing = {"step", *_STATES[bits]} - set(state)
+        if missing:
+            raise ValueError("loaded state dict lacks " + ", ".join(
+                sorted(missing)) + f" of a state of {bits} bits")
+        out = {"step": torch.as_tensor(state["step"]).to(torch.int32)}
+        if bits == 32:
+            for name in _STATES[32]:
+                out[name] = torch.empty_like(
+                    p, dtype=torch.float32, requires_grad=False).copy_(
+                        state[name])
+            return out
+        for name in ("exp_avg", "exp_avg_root"):
+            codes = state[name]
+            scales = state[name + "_scale"]
+            if codes.shape != p.shape:
+                raise ValueError(f"loaded {name} has the shape "
+                                 f"{tuple(codes.shape)}, its parameter "
+                                 f"{tuple(p.shape)}")
+            if codes.dtype != torch.float8_e4m3fn or \
+                    scales.dtype != torch.float8_e8m0fnu:
+                raise ValueError(f"loaded {name} is no 8-bit state")
+            if reference._same_layout(codes, p):
+                codes, scales = codes.clone(), scales.clone()
+            else:
+                # Groups follow the memory: another order of the dimensions
+                # (contiguous on the CPU, channels last on a GPU) has others.
+                values = torch.empty_like(
+                    p, dtype=torch.float32, requires_grad=False,
+                    device=codes.device).copy_(
+                        reference.values8(codes, scales))
+                codes, scales = reference.nearest8(
+                    values, root=name == "exp_avg_root")
+            out[name] = codes.to(p.device)
+            out[name + "_scale"] = scales.to(p.device)
+        return out

@@ -1,0 +1,500 @@
+"""Optimizer ops and AdamW on the CPU: the plain forms against 64 bits, the
+8-bit states' rounding, refusals, checkpoints, the engine."""
+
+import copy
+import io
+import math
+
+import pytest
+import torch
+
+import adamw_oracle as oracle
+from aggregathor_amd import ops
+from aggregathor_amd.graph import Engine, build_optimizer
+from aggregathor_amd.ops import adamw_reference as R
+from aggregathor_amd.optim import AdamW
+from aggregathor_amd.parallel import WorkerGroup
+from aggregathor_amd import experiments, tools
+
+SIZES = [1, 3, 31, 32, 33, 100, 257, 0]
+
+
+def _tensors(sizes, dtype=torch.float32, seed=0, scale=1.):
+    gen = torch.Generator().manual_seed(seed)
+    return [(scale * torch.randn(n, generator=gen)).to(dtype) for n in sizes]
+
+
+def _state32(params, seed=1):
+    m = [0.1 * t for t in _tensors([p.numel() for p in params], seed=seed)]
+    v = [t.square() * 0.02 for t in _tensors([p.numel() for p in params],
+                                             seed=seed + 1)]
+    return m, v
+
+
+def _state8(params, seed=1):
+    m, v = _state32(params, seed)
+    out = [R.nearest8(x, False) + R.nearest8(y.sqrt(), True)
+           for x, y in zip(m, v)]
+    return [list(column) for column in zip(*out)]
+
+
+def _steps(*counts):
+    return torch.tensor(counts, dtype=torch.int32)
+
+
+# ---------------------------------------------------------------------------- #
+# Norm
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+def test_grad_norm(dtype):
+    grads = _tensors(SIZES, dtype)
+    want = sum(float(g.double().square().sum()) for g in grads) ** .5
+    got = ops.grad_norm(grads)
+    assert got.dtype == torch.float32 and got.shape == ()
+    assert abs(float(got) - want) <= 2 * oracle.U * want
+
+
+def test_grad_norm_extremes():
+    assert float(ops.grad_norm([torch.zeros(5), torch.zeros(0)])) == 0
+    assert float(ops.grad_norm(torch.full((4,), 1e30))) == pytest.approx(2e30)
+    assert float(ops.grad_norm(torch.full((4,), 1e-30))) == pytest.approx(
+        2e-30)
+    assert math.isnan(float(ops.grad_norm([torch.tensor([float("nan"), 1.])])))
+    assert math.isinf(float(ops.grad_norm([torch.tensor([-math.inf, 1.])])))
+
+
+# ---------------------------------------------------------------------------- #
+# Step
+
+
+@pytest.mark.parametrize("max_norm", [None, 0.5, 1e6])
+@pytest.mark.parametrize("p_dtype,g_dtype", [
+    (torch.float32, torch.float32), (torch.float32, torch.bfloat16),
+    (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+def test_step32_against_64_bits(p_dtype, g_dtype, max_norm):
+    params = _tensors(SIZES, p_dtype)
+    grads = _tensors(SIZES, g_dtype, seed=5, scale=0.3)
+    m, v = _state32(params)
+    counts = [0, 1, 7, 100, 5000, 3, 2, 1]
+    steps = _steps(*counts)
+    hyper = dict(lr=1e-2, beta1=0.9, beta2=0.99, eps=1e-6, weight_decay=0.1)
+    norm, s = (None, 1.) if max_norm is None else oracle.clip_factor(
+        grads, max_norm)
+    want = [oracle.step(*x, t + 1, **hyper, s=s)
+            for *x, t in zip(params, grads, m, v, counts)]
+    plan = ops.adamw_plan(params, m, v, steps)
+    ops.adamw_step(plan, grads, **hyper, max_norm=max_norm,
+                   norm=None if norm is None else ops.grad_norm(grads))
+    assert steps.tolist() == [t + 1 for t in counts]
+    for i, (values, bounds) in enumerate(want):
+        bounds = (oracle.rounded(bounds[0], values[0], p_dtype), *bounds[1:])
+        for name, got, x, b in zip("pmv", (params[i], m[i], v[i]), values,
+                                   bounds):
+            oracle.check(got, x, b, f"{name} of {SIZES[i]}")
+
+
+def test_step8_against_64_bits():
+    params = _tensors(SIZES)
+    grads = _tensors(SIZES, seed=5, scale=0.3)
+    m, ms, r, rs = _state8(params)
+    hyper = dict(lr=1e-2, beta1=0.9, beta2=0.99, eps=1e-6, weight_decay=0.1)
+    values = [(R.values8(a, b), R.values8(c, d).square())
+              for a, b, c, d in zip(m, ms, r, rs)]
+    want = [oracle.step(p, g, *mv, 4, **hyper)
+            for p, g, mv in zip(params, grads, values)]
+    ops.adamw_step(ops.adamw8_plan(params, m, ms, r, rs, _steps(*[3] * 8)),
+                   grads, **hyper)
+    for i, (x, bounds) in enumerate(want):
+        oracle.check(params[i], x[0], bounds[0], f"p of {SIZES[i]}")
+        oracle.check8(m[i], ms[i], ops.adamw8_values(m[i], ms[i]), x[1],
+                      False, f"m of {SIZES[i]}")
+        oracle.check8(r[i], rs[i], ops.adamw8_values(r[i], rs[i]),
+                      x[2].sqrt(), True, f"r of {SIZES[i]}")
+
+
+def test_a_missing_gradient_leaves_all_as_it_was():
+    params = _tensors([5, 40, 7])
+    m, ms, r, rs = _state8(params)
+    steps = _steps(4, 4, 4)
+    before = copy.deepcopy([params[1], m[1].float(), ms[1].float(),
+                            r[1].float(), rs[1].float()])
+    ops.adamw_step(ops.adamw8_plan(params, m, ms, r, rs, steps),
+                   [torch.ones(5), None, torch.ones(7)], lr=0.1)
+    assert steps.tolist() == [5, 4, 5]
+    for x, y in zip(before, (params[1], m[1], ms[1], r[1], rs[1])):
+        assert torch.equal(x, y.float())
+
+
+def test_rounding_has_no_bias():
+    # Over all 2^16 values of the chance, the mean code is the value itself but
+    # for the chance's own grain, 2^-16 of a quantum.
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(32, generator=gen) * torch.logspace(0, -6, 32)
+    exponents = R.exponents_of(R._largest(x), False)
+    scale = 2. ** (float(exponents) - 127)
+    chance = torch.arange(65536.)
+    for value in x.tolist():
+        one = torch.full((65536,), value)
+        # The group's exponent is given, not taken from these copies.
+        codes = R.round_by_chance(one, exponents.expand(2048), chance, 0.)
+        mean = float(codes.double().mean()) * scale
+        quantum = max(2. ** (math.floor(math.log2(abs(value) / scale)) - 3),
+                      2. ** -9) * scale
+        assert abs(mean - value) <= 2. ** -16 * quantum * 1.0001
+
+
+def test_values_on_the_grid_stay():
+    grid = torch.arange(128, 256, 16.).repeat(4)  # of one group
+    codes, scales = R.nearest8(grid, False)
+    assert torch.equal(R.values8(codes, scales), grid)
+    for chance in (0., 65535.):
+        again = R.round_by_chance(grid, scales.view(torch.uint8).int(),
+                                  torch.full((32,), chance), 0.)
+        assert torch.equal(again.float(), codes.float())
+
+
+def test_random_bits_look_random():
+    bits = R.random_bits(7, 2, 5, 1 << 16, "cpu")
+    other = R.random_bits(7, 2, 6, 1 << 16, "cpu")
+    half = [(b.double() / 65536 - 0.5) for x in (bits, other)
+            for b in (x & 0xFFFF, x >> 16)]
+    # A mean of N uniform numbers is off by 1/sqrt(12 N) = 0.0011 (5 of these).
+    for h in half:
+        assert abs(float(h.mean())) < 0.006
+    for i in range(4):
+        for j in range(i):
+            c = float((half[i] * half[j]).mean() * 12)  # 1/sqrt(N) = 0.004
+            assert abs(c) < 0.02
+    assert torch.equal(R.random_bits(7, 2, 5, 100, "cpu", begin=200),
+                       bits[200:300])
+
+
+def test_state8_of_extremes():
+    inf, nan = math.inf, math.nan
+    x = torch.zeros(96)
+    x[:6] = torch.tensor([3e38, -3e38, 1e-30, inf, nan, 0.])
+    x[32:36] = torch.tensor([1e-45, -1e-40, 1e-38, 0.])
+    codes, scales = R.nearest8(x, False)
+    back = R.values8(codes, scales)
+    assert back[:2].tolist() == pytest.approx([3e38, -3e38], rel=2. ** -4)
+    assert back[2] == 0 and back[5] == 0
+    assert back[3].isnan() and back[4].isnan()
+    # Half a quantum of the least scale, 2^-120 2^-9.
+    assert (back[32:36] - x[32:36]).abs().max() <= 2. ** -130 * 1.01
+    assert torch.equal(back[64:], torch.zeros(32))
+
+
+def test_roots_never_become_zero():
+    params = [torch.zeros(64)]
+    m, ms, r, rs = _state8(params, seed=9)
+    grad = torch.full((64,), 1e-12)
+    grad[0] = 1e3
+    steps = _steps(0)
+    state = ops.adamw8_state(params[0])
+    plan = ops.adamw8_plan(params, [state[0]], [state[1]], [state[2]],
+                           [state[3]], steps)
+    for _ in range(4):
+        ops.adamw_step(plan, [grad], lr=1e-3)
+        root = ops.adamw8_values(state[2], state[3])
+        assert bool((root > 0).all())
+        # Each step moves a parameter by lr at most times what the momenta
+        # allow, (1 - beta1) / sqrt(1 - beta2) = 3.2: nothing is thrown.
+    assert float(params[0].abs().max()) < 4 * 1e-3 * 3.3
+
+
+def test_nan_and_infinity_stay_where_they_are():
+    for make in ("32", "8"):
+        params = [torch.ones(64)]
+        grad = torch.ones(64)
+        grad[3], grad[40] = math.nan, math.inf
+        if make == "32":
+            plan = ops.adamw_plan(params, [torch.zeros(64)],
+                                  [torch.zeros(64)], _steps(0))
+        else:
+            plan = ops.adamw8_plan(
+                params, *[[x] for x in ops.adamw8_state(params[0])], _steps(0))
+        for _ in range(2):
+            ops.adamw_step(plan, [grad], lr=1e-3)
+        bad = torch.zeros(64, dtype=torch.bool)
+        bad[[3, 40]] = True
+        assert torch.equal(~params[0].isfinite(), bad)
+
+
+def test_averages_follow_in_8_bits():
+    # r of a constant gradient: with unbiased rounding the mean over many
+    # elements follows sqrt(1 - beta2^t) |g|, though one step moves r by far
+    # less than half a quantum. Its quantum is at most an eighth, so one
+    # rounding's spread is at most r / 16; a rounding lasts 1/(1 - beta2^.5)
+    # steps or so, so t of them add up to at most sqrt(t) r / 16 = 0.9 r each,
+    # and the mean over 32768 elements to 0.005 r: 4 of these, and as much for
+    # the bias of a square's root (half the variance).
+    n, t = 32768, 200
+    params = [torch.zeros(n)]
+    state = ops.adamw8_state(params[0])
+    plan = ops.adamw8_plan(params, *[[x] for x in state], _steps(0), seed=11)
+    grad = torch.full((n,), 0.37)
+    for _ in range(t):
+        ops.adamw_step(plan, [grad], lr=1e-5)
+    root = float(ops.adamw8_values(state[2], state[3]).mean())
+    assert root == pytest.approx(0.37 * (1 - 0.999 ** t) ** .5, rel=0.04)
+    m = float(ops.adamw8_values(state[0], state[1]).mean())
+    assert m == pytest.approx(0.37, rel=0.01)
+
+
+# ---------------------------------------------------------------------------- #
+# Refusals
+
+
+def _plan_args(n=40, bits=8):
+    p = torch.zeros(n)
+    if bits == 32:
+        return [[p], [torch.zeros(n)], [torch.zeros(n)], _steps(0)]
+    return [[p], *[[x] for x in ops.adamw8_state(p)], _steps(0)]
+
+
+@pytest.mark.parametrize("bits,place,value", [
+    (32, 0, [torch.zeros(40, dtype=torch.float64)]),
+    (32, 0, [torch.zeros(80)[::2]]),
+    (32, 0, []),
+    (32, 1, [torch.zeros(41)]),
+    (32, 1, [torch.zeros(40, dtype=torch.bfloat16)]),
+    (32, 1, []),
+    (32, 2, [torch.zeros(80)[::2]]),
+    (32, 3, torch.zeros(1)),
+    (32, 3, torch.zeros(2, dtype=torch.int32)),
+    (8, 1, [torch.zeros(40)]),
+    (8, 2, [torch.zeros(2, dtype=torch.uint8)]),
+    (8, 2, [torch.zeros(1, dtype=torch.uint8).view(torch.float8_e8m0fnu)]),
+    (8, 4, [torch.zeros(3, dtype=torch.uint8).view(torch.float8_e8m0fnu)]),
+])
+def test_plan_refuses(bits, place, value):
+    args = _plan_args(bits=bits)
+    make = ops.adamw_plan if bits == 32 else ops.adamw8_plan
+    make(*args)
+    args[place] = value
+    with pytest.raises(RuntimeError):
+        make(*args)
+
+
+def test_plan_refuses_shared_memory():
+    flat = torch.zeros(100)
+    other = lambda: [torch.zeros(40), torch.zeros(40)]  # noqa: E731
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.adamw_plan([flat[:40], flat[39:79]], other(), other(),
+                       _steps(0, 0))
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.adamw_plan([flat[:40]], [flat[20:60]], [torch.zeros(40)],
+                       _steps(0))
+    ops.adamw_plan([flat[:40], flat[40:80]], other(), other(), _steps(0, 0))
+
+
+@pytest.mark.parametrize("change", [
+    dict(grads=[]), dict(grads=[torch.zeros(41)]),
+    dict(grads=[torch.zeros(40, dtype=torch.float64)]),
+    dict(grads=[torch.zeros(40).to_sparse()]),
+    dict(lr=-1.), dict(lr=math.nan), dict(lr=math.inf), dict(beta1=1.),
+    dict(beta2=-0.1), dict(eps=0.), dict(weight_decay=math.nan),
+    dict(norm=torch.ones(())), dict(max_norm=1.),
+    dict(norm=torch.ones(()), max_norm=0.),
+    dict(norm=torch.ones((), dtype=torch.float64), max_norm=1.),
+    dict(norm=torch.ones(2), max_norm=1.)])
+def test_step_refuses(change):
+    args = _plan_args(bits=32)
+    plan = ops.adamw_plan(*args)
+    with pytest.raises(RuntimeError):
+        ops.adamw_step(plan, **{"grads": [torch.ones(40)], "lr": 0.1,
+                                **change})
+    assert int(args[3]) == 0 and torch.equal(args[0][0], torch.zeros(40))
+
+
+def test_step_refuses_what_it_writes_as_input():
+    args = _plan_args(bits=32)
+    plan = ops.adamw_plan(*args)
+    for shared in (args[0][0], args[1][0]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.adamw_step(plan, [shared], lr=0.1)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        ops.adamw_step(plan, [torch.ones(40)], lr=0.1,
+                       norm=args[2][0][5], max_norm=1.)
+
+
+def test_16_bit_parameters_refuse_other_gradients():
+    p = torch.zeros(8, dtype=torch.bfloat16)
+    plan = ops.adamw_plan([p], [torch.zeros(8)], [torch.zeros(8)], _steps(0))
+    for dtype in (torch.float32, torch.float16):
+        with pytest.raises(RuntimeError):
+            ops.adamw_step(plan, [torch.ones(8, dtype=dtype)], lr=0.1)
+
+
+def test_grad_norm_refuses():
+    for bad in ([], [torch.zeros(3, dtype=torch.int32)],
+                [torch.zeros(3).to_sparse()]):
+        with pytest.raises(RuntimeError):
+            ops.grad_norm(bad)
+
+
+# ---------------------------------------------------------------------------- #
+# Optimizer
+
+
+def _model(channels_last=False, seed=0):
+    torch.manual_seed(seed)
+    model = torch.nn.Sequential(torch.nn.Conv2d(3, 8, 3), torch.nn.Flatten(),
+                                torch.nn.Linear(8 * 36, 10))
+    return model.to(memory_format=torch.channels_last) if channels_last \
+        else model
+
+
+def _train(model, optimizer, steps, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    for _ in range(steps):
+        optimizer.zero_grad()
+        model(torch.randn(4, 3, 8, 8, generator=gen)).square().mean().backward()
+        optimizer.step()
+
+
+def test_optimizer_matches_torch():
+    mine, other = _model(), _model()
+    a = AdamW(mine.parameters(), lr=1e-3, weight_decay=0.1)
+    b = torch.optim.AdamW(other.parameters(), lr=1e-3, weight_decay=0.1)
+    _train(mine, a, 10)
+    _train(other, b, 10)
+    for p, q in zip(mine.parameters(), other.parameters()):
+        # Ten steps of 1e-3, each off by 20 u of itself or so, and by the
+        # gradients' own differences.
+        torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-6)
+
+
+def test_optimizer_clips_as_torch_does():
+    mine, other = _model(), _model()
+    a = AdamW(mine.parameters(), max_norm=0.01)
+    b = torch.optim.AdamW(other.parameters())
+    x = torch.randn(4, 3, 8, 8)
+    for model in (mine, other):
+        model(x).square().mean().backward()
+    norm = torch.nn.utils.clip_grad_norm_(other.parameters(), 0.01)
+    assert float(norm) > 0.01
+    a.step()
+    b.step()
+    for p, q in zip(mine.parameters(), other.parameters()):
+        # clip_grad_norm_ adds 1e-6 to the norm; m / sqrt(v) hardly sees it.
+        torch.testing.assert_close(p, q, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("channels_last", [False, True])
+def test_checkpoint_goes_on_alike(bits, channels_last):
+    whole = _model(channels_last)
+    opt = AdamW(whole.parameters(), state_bits=bits, rounding_seed=3)
+    _train(whole, opt, 3)
+    file = io.BytesIO()
+    torch.save({"m": whole.state_dict(), "o": opt.state_dict()}, file)
+    file.seek(0)
+    saved = torch.load(file, weights_only=True)
+    again = _model(channels_last, seed=9)
+    again.load_state_dict(saved["m"])
+    opt2 = AdamW(again.parameters(), rounding_seed=3)
+    opt2.load_state_dict(saved["o"])
+    copied = copy.deepcopy((whole, opt))
+    for model, optimizer in ((whole, opt), (again, opt2), copied):
+        _train(model, optimizer, 3, seed=1)
+    for p, q, w in zip(whole.parameters(), again.parameters(),
+                       copied[0].parameters()):
+        assert torch.equal(p, q) and torch.equal(p, w)
+    assert int(opt2.state[next(again.parameters())]["step"]) == 6
+
+
+def test_checkpoint_into_another_memory_order():
+    first = _model(True)
+    opt = AdamW(first.parameters(), state_bits=8)
+    _train(first, opt, 3)
+    second = _model(False)
+    second.load_state_dict(first.state_dict())
+    opt2 = AdamW(second.parameters(), state_bits=8)
+    opt2.load_state_dict(opt.state_dict())
+    for p, q in zip(first.parameters(), second.parameters()):
+        for name in ("exp_avg", "exp_avg_root"):
+            x, y = (ops.adamw8_values(s[name], s[name + "_scale"])
+                    for s in (opt.state[p], opt2.state[q]))
+            # To nearest: half of e4m3's step, or of its least step.
+            assert bool(((x - y).abs() <= 2. ** -4 * x.abs()
+                         + 2. ** -18 * x.abs().max()).all())
+    _train(second, opt2, 1)
+
+
+def test_loads_torchs_state():
+    first, second = _model(), _model()
+    opt = torch.optim.AdamW(first.parameters())
+    _train(first, opt, 3)
+    second.load_state_dict(first.state_dict())
+    opt2 = AdamW(second.parameters())
+    opt2.load_state_dict(opt.state_dict())
+    _train(first, opt, 2, seed=1)
+    _train(second, opt2, 2, seed=1)
+    for p, q in zip(first.parameters(), second.parameters()):
+        torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-6)
+
+
+def test_optimizer_refuses():
+    model = _model()
+    with pytest.raises(tools.UserException):
+        AdamW(model.parameters(), state_bits=16)
+    with pytest.raises(tools.UserException):
+        AdamW(model.parameters(), max_norm=0.)
+    opt = AdamW(model.parameters())
+    _train(model, opt, 1)
+    state = opt.state_dict()
+    state["param_groups"][0]["state_bits"] = 8
+    with pytest.raises(ValueError):
+        AdamW(model.parameters()).load_state_dict(state)
+    with pytest.raises(ValueError):
+        AdamW(list(model.parameters())[1:]).load_state_dict(opt.state_dict())
+
+
+def test_groups_with_their_own_settings():
+    model = _model()
+    params = list(model.parameters())
+    opt = AdamW([{"params": params[:2], "state_bits": 8, "lr": 0.},
+                 {"params": params[2:]}], lr=1e-2)
+    before = [p.detach().clone() for p in params]
+    _train(model, opt, 1)
+    assert all(torch.equal(a, b) for a, b in zip(before[:2], params[:2]))
+    assert not any(torch.equal(a, b) for a, b in zip(before[2:], params[2:]))
+    assert "exp_avg_root" in opt.state[params[0]]
+    opt.state.clear()
+    _train(model, opt, 1)
+    assert int(opt.state[params[0]]["step"]) == 1
+
+
+def test_registry():
+    p = [torch.nn.Parameter(torch.zeros(4))]
+    opt = build_optimizer("adamw", ["state-bits:8", "clip-norm:2",
+                                    "weight-decay:0.5", "rounding-seed:4"],
+                          p, 0.25)
+    assert isinstance(opt, AdamW) and opt.max_norm == 2
+    assert opt.rounding_seed == 4
+    group = opt.param_groups[0]
+    assert group["state_bits"] == 8 and group["weight_decay"] == 0.5
+    assert group["lr"] == 0.25
+    assert build_optimizer("adamw", [], p, 1.).max_norm is None
+
+
+@pytest.mark.parametrize("args", [[], ["state-bits:8", "clip-norm:0.5"]])
+def test_engine_steps_and_resumes(args):
+    def engine():
+        exp = experiments.instantiate("mnist", ["batch-size:16"])
+        return Engine(exp, "krum", WorkerGroup(5, device="cpu"), nbbyzwrks=1,
+                      optimizer="adamw", optimizer_args=args, seed=5)
+    one, two = engine(), engine()
+    for _ in range(3):
+        assert math.isfinite(one.step())
+    file = io.BytesIO()
+    torch.save(one.state_dict(), file)
+    file.seek(0)
+    two.load_state_dict(torch.load(file, weights_only=True))
+    one.step()
+    two.step()
+    for p, q in zip(one.params, two.params):
+        assert torch.equal(p, q)
