@@ -45,16 +45,11 @@ struct Chunk {
   int index;
 };
 
-// The gradients of a launch: null where a tensor has none, and two bits each
-// for their types.
+// The gradients of a launch: null where a tensor has none (not where it has no
+// elements), and two bits each for their types.
 struct Grads {
   const void* g[kMaxTensors];
   uint32_t types[kMaxTensors / 16];
-};
-
-// A bit for each tensor of a launch that has a gradient.
-struct Present {
-  uint64_t bits[kMaxTensors / 64];
 };
 
 struct Hyper {
@@ -66,15 +61,17 @@ struct Hyper {
 // Whether update() has a form for parameters of type p and gradients of type g.
 bool supported(int p, int g);
 
-// steps[i] += 1 and coefs[i] = {lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)} for
-// those of `count` tensors that are present.
-void begin_step(int* steps, float2* coefs, const Present& present, int count,
-                const Hyper& hyper, hipStream_t stream);
+// Arrivals of a launch's workgroups: one counter for all, then kTicketLines for
+// a part of them each, every one on a cache line of its own. Zero before the
+// first launch; each launch leaves them so.
+constexpr int kTicketLines = 32;
+constexpr int kTicketInts = 32 * (kTicketLines + 1);
 
-// One AdamW step of the chunks [0, nchunks); grads.g[i] belongs to tensor
-// first + i of `tensors`, `steps` and `coefs`.
+// One AdamW step of the chunks [0, nchunks) of the tensors [first, first +
+// count) of `tensors` and `steps`: steps[i] += 1 for those that are present.
+// grads.g[i] belongs to tensor first + i, whose chunks are the tensor's whole.
 void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
-            int first, const int* steps, const float2* coefs,
+            int first, int count, int* steps, unsigned* tickets,
             const Grads& grads, const Hyper& hyper, hipStream_t stream);
 
 // Spans of elements that lie back to back in memory: start[i] is the first

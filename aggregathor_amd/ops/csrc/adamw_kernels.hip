@@ -289,36 +289,78 @@ __device__ __forceinline__ void update_tensor(const Tensor& t, const void* grad,
 }
 
 struct Scalars {
-  float beta1, rest1, beta2, rest2, eps, keep, max_norm;
+  double beta1, beta2;
+  float lr, rest1, rest2, eps, keep, max_norm;
   const float* norm;
 };
+
+// rate = lr / (1 - beta1^t) and unbias = 1 / sqrt(1 - beta2^t), the powers by
+// squaring in 64 bits (1 - beta^t loses what 32 hold while it is near zero):
+// beta1's in even lanes, beta2's in odd ones.
+__device__ __forceinline__ void bias(const Scalars& s, uint32_t t, Common& k) {
+  const bool odd = threadIdx.x & 1;
+  double x = odd ? s.beta2 : s.beta1, power = 1.0;
+  for (; t != 0; t >>= 1) {
+    if (t & 1) power *= x;
+    x *= x;
+  }
+  const float rest = (float)(1.0 - power);
+  const float out = odd ? 1.f / sqrtf(rest) : s.lr / rest;
+  k.rate = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(out), 0));
+  k.unbias =
+      __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(out), 1));
+}
+
+// Step counts are read by all workgroups and written once, by the first wave of
+// the last workgroup that has read them. (A launch of its own for that took 3 to
+// 4 us a step; this takes 0.6.) One address takes an arrival in 12 ns, so they
+// arrive at 32, and the last of each of these at one. Counters wrap by
+// themselves to the zero that the next launch needs.
+__device__ __forceinline__ bool last_to_arrive(unsigned* tickets) {
+  __syncthreads();  // all four waves have read
+  bool last = false;
+  if (threadIdx.x == 0) {
+    const unsigned groups = gridDim.x, line = blockIdx.x % kTicketLines;
+    const unsigned lines = groups < kTicketLines ? groups : kTicketLines;
+    const unsigned of_line = (groups - line + kTicketLines - 1) / kTicketLines;
+    if (atomicInc(tickets + 32 * (1 + line), of_line - 1) == of_line - 1)
+      last = atomicInc(tickets, lines - 1) == lines - 1;
+  }
+  return threadIdx.x < 64 && __builtin_amdgcn_readfirstlane(last);
+}
 
 template <int Bits>
 __global__ __launch_bounds__(kBlock) void update_kernel(
     const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
-    int first, const int* __restrict__ steps,
-    const float2* __restrict__ coefs, const Grads grads, const Scalars s) {
-  const Chunk chunk = chunks[blockIdx.x];
+    long nchunks, int first, int count, int* steps, unsigned* tickets,
+    const Grads grads, const Scalars s) {
+  // A launch without chunks has one workgroup that counts.
+  const bool some = blockIdx.x < nchunks;
+  const Chunk chunk = some ? chunks[blockIdx.x] : Chunk{first, 0};
   const int at = chunk.tensor - first;
   const void* const grad = grads.g[at];
-  if (grad == nullptr) return;
+  const int step = __hip_atomic_load(steps + chunk.tensor, __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT) + 1;
+  if (last_to_arrive(tickets)) {
+    for (int i = threadIdx.x; i < count; i += 64)
+      if (grads.g[i] != nullptr) steps[first + i] += 1;
+  }
+  if (!some || grad == nullptr) return;
   const Tensor t = tensors[chunk.tensor];
-  const float2 coef = coefs[chunk.tensor];
   Common k;
   k.clip = 1.f;
   if (s.norm != nullptr) {
     const float norm = *s.norm;
     k.clip = norm <= s.max_norm ? 1.f : s.max_norm / norm;
   }
-  k.beta1 = s.beta1;
+  k.beta1 = (float)s.beta1;
   k.rest1 = s.rest1;
-  k.beta2 = s.beta2;
+  k.beta2 = (float)s.beta2;
   k.rest2 = s.rest2;
   k.eps = s.eps;
   k.keep = s.keep;
-  k.rate = coef.x;
-  k.unbias = coef.y;
-  k.key = Bits == 8 ? mix(t.key + (uint32_t)steps[chunk.tensor]) : 0;
+  bias(s, (uint32_t)step, k);
+  k.key = Bits == 8 ? mix(t.key + (uint32_t)step) : 0;
   const long start = (long)chunk.index * kChunk;
   const uint32_t gt = (grads.types[at / 16] >> (2 * (at % 16))) & 3;
   switch (t.type * 4 + gt) {
@@ -334,18 +376,6 @@ __global__ __launch_bounds__(kBlock) void update_kernel(
     case kF16 * 4 + kF16:
       return update_tensor<Bits, __half, __half>(t, grad, start, k);
   }
-}
-
-__global__ __launch_bounds__(kMaxTensors) void begin_step_kernel(
-    int* steps, float2* coefs, Present present, int count, double lr,
-    double beta1, double beta2) {
-  const int i = threadIdx.x;
-  if (i >= count || !(present.bits[i / 64] >> (i % 64) & 1)) return;
-  const int t = steps[i] + 1;
-  steps[i] = t;
-  // In 64 bits: 1 - beta^t loses what 32 hold when it is near zero.
-  coefs[i] = make_float2((float)(lr / (1.0 - pow(beta1, (double)t))),
-                         (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))));
 }
 
 // ---------------------------------------------------------------------------
@@ -428,29 +458,25 @@ __global__ __launch_bounds__(kBlock) void norm_finish_kernel(
 
 bool supported(int p, int g) { return p == g || p == kF32; }
 
-void begin_step(int* steps, float2* coefs, const Present& present, int count,
-                const Hyper& h, hipStream_t stream) {
-  begin_step_kernel<<<1, kMaxTensors, 0, stream>>>(steps, coefs, present, count,
-                                                   h.lr, h.beta1, h.beta2);
-}
-
 void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
-            int first, const int* steps, const float2* coefs,
+            int first, int count, int* steps, unsigned* tickets,
             const Grads& grads, const Hyper& h, hipStream_t stream) {
-  const Scalars s = {(float)h.beta1,
+  const Scalars s = {h.beta1,
+                     h.beta2,
+                     (float)h.lr,
                      (float)(1.0 - h.beta1),
-                     (float)h.beta2,
                      (float)(1.0 - h.beta2),
                      (float)h.eps,
                      (float)(1.0 - h.lr * h.weight_decay),
                      (float)h.max_norm,
                      h.norm};
+  const dim3 grid((unsigned)(nchunks > 0 ? nchunks : 1));
   if (bits == 8)
-    update_kernel<8><<<dim3((unsigned)nchunks), kBlock, 0, stream>>>(
-        tensors, chunks, first, steps, coefs, grads, s);
+    update_kernel<8><<<grid, kBlock, 0, stream>>>(
+        tensors, chunks, nchunks, first, count, steps, tickets, grads, s);
   else
-    update_kernel<32><<<dim3((unsigned)nchunks), kBlock, 0, stream>>>(
-        tensors, chunks, first, steps, coefs, grads, s);
+    update_kernel<32><<<grid, kBlock, 0, stream>>>(
+        tensors, chunks, nchunks, first, count, steps, tickets, grads, s);
 }
 
 int norm_blocks(const Spans& spans) {

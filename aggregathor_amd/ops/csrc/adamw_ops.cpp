@@ -158,12 +158,12 @@ class Plan {
     const auto stream = current.stream();
     if (capturing()) {
       if (!captured_)
-        for (const Tensor& t : {device_table_, device_chunks_, coefs_})
+        for (const Tensor& t : {device_table_, device_chunks_, tickets_})
           captured_tables().push_back(t);
       captured_ = true;
     } else if (current != laid_out_on_) {
       // The allocator must not give these to others before this step is done.
-      for (const Tensor& t : {device_table_, device_chunks_, coefs_})
+      for (const Tensor& t : {device_table_, device_chunks_, tickets_})
         t.record_stream(
             c10::hip::HIPStreamMasqueradingAsCUDA(current).unwrap());
     }
@@ -171,32 +171,27 @@ class Plan {
         reinterpret_cast<const adamw::Tensor*>(device_table_.data_ptr());
     const auto* chunks =
         reinterpret_cast<const adamw::Chunk*>(device_chunks_.data_ptr());
-    auto* coefs = reinterpret_cast<float2*>(coefs_.data_ptr());
+    auto* tickets = reinterpret_cast<unsigned*>(tickets_.data_ptr());
     int* steps = steps_.data_ptr<int>();
     for (size_t first = 0; first < count; first += adamw::kMaxTensors) {
       const size_t last = std::min(count, first + adamw::kMaxTensors);
       adamw::Grads g{};
-      adamw::Present present{};
       bool any = false;
       for (size_t i = first; i < last; ++i) {
         if (!held[i].defined()) continue;
         const size_t k = i - first;
         any = true;
-        g.g[k] = held[i].data_ptr();
+        // A tensor of no elements has a gradient all the same: any address.
+        g.g[k] = held[i].numel() > 0 ? held[i].data_ptr() : (const void*)tensors;
         g.types[k / 16] |= (uint32_t)types[i] << (2 * (k % 16));
-        present.bits[k / 64] |= 1ull << (k % 64);
       }
       if (!any) continue;
-      adamw::begin_step(steps + first, coefs + first, present,
-                        (int)(last - first), hyper, stream);
-      C10_HIP_CHECK(hipGetLastError());
       const int64_t begin = chunk_start_[first];
-      const int64_t nchunks = chunk_start_[last] - begin;
-      if (nchunks > 0) {
-        adamw::update(bits_, tensors, chunks + begin, nchunks, (int)first,
-                      steps, coefs, g, hyper, stream);
-        C10_HIP_CHECK(hipGetLastError());
-      }
+      adamw::update(bits_, tensors, chunks + begin, chunk_start_[last] - begin,
+                    (int)first, (int)(last - first), steps,
+                    tickets + first / adamw::kMaxTensors * adamw::kTicketInts,
+                    g, hyper, stream);
+      C10_HIP_CHECK(hipGetLastError());
     }
     // What autograd has saved of the parameters is out of date.
     for (size_t i = 0; i < count; ++i)
@@ -312,12 +307,15 @@ class Plan {
       TORCH_CHECK(written[i - 1].hi <= written[i].lo,
                   "adamw: parameters, states and steps share memory");
     c10::DeviceGuard guard(device);
+    const int64_t launches =
+        (int64_t)(count + adamw::kMaxTensors - 1) / adamw::kMaxTensors;
+    tickets_ = torch::zeros(
+        {launches * adamw::kTicketInts},
+        torch::TensorOptions().device(device).dtype(torch::kInt32));
+    // Uploads wait for the stream, so another one may use all of these next.
     device_table_ = upload(table, device);
     if (chunks.empty()) chunks.push_back({0, 0});
     device_chunks_ = upload(chunks, device);
-    coefs_ = torch::empty({(int64_t)count, 2},
-                          torch::TensorOptions().device(device).dtype(
-                              torch::kFloat32));
     laid_out_on_ = c10::hip::getCurrentHIPStream();
     steps_at_ = steps_.data_ptr();
     table_ = std::move(table);
@@ -344,7 +342,7 @@ class Plan {
   std::vector<adamw::Tensor> table_;
   std::vector<int64_t> chunk_start_;
   std::vector<Range> written_;
-  Tensor device_table_, device_chunks_, coefs_;
+  Tensor device_table_, device_chunks_, tickets_;
   c10::hip::HIPStream laid_out_on_ = c10::hip::getDefaultHIPStream();
   const void* steps_at_ = nullptr;
   bool captured_ = false;
