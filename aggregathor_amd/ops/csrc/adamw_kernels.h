@@ -24,25 +24,23 @@ constexpr int kMaxSpans = 160;
 constexpr int kNormBlocks = 2048;
 constexpr int kNormChunkBytes = 16384;
 
-// One parameter tensor of a plan. 32-bit states: m and r point to floats (r to
-// the mean square itself), ms and rs are null. 8-bit states: m and r point to
-// e4m3 codes (r to those of the mean square's root), ms and rs to their groups'
-// biased exponents.
-struct Tensor {
+// What one workgroup updates: `left` elements of a tensor from the element
+// `start` on (a multiple of kChunk), where the pointers point. All that it needs
+// is in one place, so that its first loads of data wait for one load only.
+// 32-bit states: m and r point to floats (r to the mean square itself), ms and
+// rs are null. 8-bit states: m and r point to e4m3 codes (r to those of the mean
+// square's root), ms and rs to their groups' biased exponents.
+struct Work {
   void* p;
   void* m;
   void* r;
   uint8_t* ms;
   uint8_t* rs;
-  long n;
+  long start;
+  int tensor;
+  int left;
   uint32_t key;  // of the rounding's random bits
   int type;      // of p
-};
-
-// Which part of which tensor a workgroup updates.
-struct Chunk {
-  int tensor;
-  int index;
 };
 
 // The gradients of a launch: null where a tensor has none (not where it has no
@@ -67,12 +65,12 @@ bool supported(int p, int g);
 constexpr int kTicketLines = 32;
 constexpr int kTicketInts = 32 * (kTicketLines + 1);
 
-// One AdamW step of the chunks [0, nchunks) of the tensors [first, first +
-// count) of `tensors` and `steps`: steps[i] += 1 for those that are present.
-// grads.g[i] belongs to tensor first + i, whose chunks are the tensor's whole.
-void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
-            int first, int count, int* steps, unsigned* tickets,
-            const Grads& grads, const Hyper& hyper, hipStream_t stream);
+// One AdamW step of the tensors [first, first + count): steps[i] += 1 for those
+// that have a gradient. work[0..nwork) is all that there is to do for them, and
+// grads.g[i] belongs to tensor first + i.
+void update(int bits, const Work* work, long nwork, int first, int count,
+            int* steps, unsigned* tickets, const Grads& grads,
+            const Hyper& hyper, hipStream_t stream);
 
 // Spans of elements that lie back to back in memory: start[i] is the first
 // chunk (of kNormChunkBytes) of span i within the launch, start[count] their

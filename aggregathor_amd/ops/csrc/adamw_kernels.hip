@@ -26,8 +26,6 @@
 // operation (no contraction into fused multiply-adds), so that states can be
 // compared with another implementation's bit by bit.
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include "adamw_kernels.h"
@@ -44,68 +42,88 @@ constexpr int kQuads = kChunk / (4 * kBlock);  // quads of a thread
 // Four elements of T. Tensors start anywhere (a gradient is a view into the
 // flat gradient), so a quad is only aligned like its element: gfx950 loads and
 // stores it in one instruction all the same.
+typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t codes4 __attribute__((aligned(1)));
+
+// Pointers that come out of memory could be to anything for all the compiler
+// knows; these are to global memory, which has loads and stores of its own.
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Quad {
-  T v[4];
+using Global = __attribute__((address_space(1))) T*;
+
+struct F32 {
+  typedef float Elem;
+  typedef f32x4 Quad;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
 };
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__hip_bfloat16 v) {
-  return __bfloat162float(v);
-}
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+struct BF16 {
+  typedef uint16_t Elem;
+  typedef u16x4 Quad;
+  static __device__ __forceinline__ float get(uint16_t v) {
+    return __uint_as_float((uint32_t)v << 16);
+  }
+  static __device__ __forceinline__ uint16_t put(float v) {
+    return __builtin_bit_cast(uint16_t, (__bf16)v);
+  }
+};
 
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) {
-  return __float2bfloat16(v);
-}
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) {
-  return __float2half(v);
-}
+struct F16 {
+  typedef uint16_t Elem;
+  typedef u16x4 Quad;
+  static __device__ __forceinline__ float get(uint16_t v) {
+    return (float)__builtin_bit_cast(_Float16, v);
+  }
+  static __device__ __forceinline__ uint16_t put(float v) {
+    return __builtin_bit_cast(uint16_t, (_Float16)v);
+  }
+};
 
-// Loads elements [i, i + 4) below n; those behind it are zero.
+// Elements [i, i + 4) below n; those behind it are zero.
 template <bool Full, typename T>
-__device__ __forceinline__ void load4(const T* base, long i, long n,
-                                      float (&out)[4]) {
+__device__ __forceinline__ typename T::Quad load4(
+    Global<const typename T::Elem> base, int i, int n) {
+  typename T::Quad q;
   if (Full || i + 4 <= n) {
-    Quad<T> q = *reinterpret_cast<const Quad<T>*>(base + i);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) out[c] = to_f32(q.v[c]);
+    q = __builtin_nontemporal_load(
+        (Global<const typename T::Quad>)(base + i));
   } else {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) out[c] = i + c < n ? to_f32(base[i + c]) : 0.f;
+    for (int c = 0; c < 4; ++c) q[c] = i + c < n ? base[i + c] : 0;
   }
+  return q;
 }
 
 template <bool Full, typename T>
-__device__ __forceinline__ void store4(T* base, long i, long n,
+__device__ __forceinline__ void store4(Global<typename T::Elem> base, int i, int n,
                                        const float (&x)[4]) {
-  if (Full || i + 4 <= n) {
-    Quad<T> q;
+  typename T::Quad q;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) q.v[c] = from_f32<T>(x[c]);
-    *reinterpret_cast<Quad<T>*>(base + i) = q;
+  for (int c = 0; c < 4; ++c) q[c] = T::put(x[c]);
+  if (Full || i + 4 <= n) {
+    __builtin_nontemporal_store(
+        q, (Global<typename T::Quad>)(base + i));
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (i + c < n) base[i + c] = from_f32<T>(x[c]);
+      if (i + c < n) base[i + c] = q[c];
   }
 }
 
-// Four codes as one word, and back.
-struct __attribute__((packed, aligned(1))) Word {
-  uint32_t v;
-};
+template <typename T>
+__device__ __forceinline__ void widen(typename T::Quad q, float (&out)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) out[c] = T::get(q[c]);
+}
 
+// Four codes as one word.
 template <bool Full>
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* base, long i,
-                                               long n) {
-  if (Full || i + 4 <= n) return reinterpret_cast<const Word*>(base + i)->v;
+__device__ __forceinline__ uint32_t load_codes(Global<const uint8_t> base, int i,
+                                               int n) {
+  if (Full || i + 4 <= n)
+    return __builtin_nontemporal_load(
+        (Global<const codes4>)(base + i));
   uint32_t w = 0;
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -114,10 +132,10 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* base, long i,
 }
 
 template <bool Full>
-__device__ __forceinline__ void store_codes(uint8_t* base, long i, long n,
+__device__ __forceinline__ void store_codes(Global<uint8_t> base, int i, int n,
                                             uint32_t w) {
   if (Full || i + 4 <= n) {
-    reinterpret_cast<Word*>(base + i)->v = w;
+    __builtin_nontemporal_store(w, (Global<codes4>)(base + i));
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -219,75 +237,6 @@ __device__ __forceinline__ void move(const Common& k, const float (&m)[4],
     p[c] = p[c] * k.keep - k.rate * (m[c] / (root[c] * k.unbias + k.eps));
 }
 
-template <int Bits, typename P, typename G, bool Full>
-__device__ __forceinline__ void update_chunk(const Tensor& t, const G* grad,
-                                             long start, const Common& k) {
-  P* const param = reinterpret_cast<P*>(t.p);
-  const long n = t.n;
-#pragma unroll
-  for (int q = 0; q < kQuads; ++q) {
-    const long i = start + 4 * ((long)q * kBlock + threadIdx.x);
-    float p[4], g[4], m[4], v[4], root[4];
-    load4<Full>(param, i, n, p);
-    load4<Full>(grad, i, n, g);
-    if constexpr (Bits == 32) {
-      float* const mp = reinterpret_cast<float*>(t.m);
-      float* const vp = reinterpret_cast<float*>(t.r);
-      load4<Full>(mp, i, n, m);
-      load4<Full>(vp, i, n, v);
-      moments(k, g, m, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
-      store4<Full>(mp, i, n, m);
-      store4<Full>(vp, i, n, v);
-    } else {
-      uint8_t* const mc = reinterpret_cast<uint8_t*>(t.m);
-      uint8_t* const rc = reinterpret_cast<uint8_t*>(t.r);
-      const long group = i / kGroup;
-      const bool some = Full || i < n;
-      decode(load_codes<Full>(mc, i, n), some ? pow2(t.ms[group]) : 0.f, m);
-      decode(load_codes<Full>(rc, i, n), some ? pow2(t.rs[group]) : 0.f, root);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = root[c] * root[c];
-      moments(k, g, m, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
-
-      // All eight lanes of a group come here, also those behind the end.
-      const uint32_t em = max8(top_bits(m)) >> 23;
-      const uint32_t ev = max8(top_bits(v)) >> 23;
-      const uint32_t sm = em < 14 ? 7 : em - 7;
-      const uint32_t sr = (uint32_t)(((int)ev - 127) >> 1) + 120;
-      const float im = pow2(254 - sm), ir = pow2(254 - sr);
-      float zm[4], zr[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t h = mix((uint32_t)(i + c) ^ (k.key + 0x9E3779B9u * (uint32_t)(i >> 32)));
-        zm[c] = round_by_chance(m[c], im, h & 0xFFFFu, 0.f);
-        zr[c] = round_by_chance(root[c], ir, h >> 16, 1.f);
-      }
-      store_codes<Full>(mc, i, n, encode(zm));
-      store_codes<Full>(rc, i, n, encode(zr));
-      if (some && threadIdx.x % (kGroup / 4) == 0) {
-        t.ms[group] = (uint8_t)sm;
-        t.rs[group] = (uint8_t)sr;
-      }
-    }
-    move(k, m, root, p);
-    store4<Full>(param, i, n, p);
-  }
-}
-
-template <int Bits, typename P, typename G>
-__device__ __forceinline__ void update_tensor(const Tensor& t, const void* grad,
-                                              long start, const Common& k) {
-  const G* const g = reinterpret_cast<const G*>(grad);
-  if (start + kChunk <= t.n)
-    update_chunk<Bits, P, G, true>(t, g, start, k);
-  else
-    update_chunk<Bits, P, G, false>(t, g, start, k);
-}
-
 struct Scalars {
   double beta1, beta2;
   float lr, rest1, rest2, eps, keep, max_norm;
@@ -297,56 +246,8 @@ struct Scalars {
 // rate = lr / (1 - beta1^t) and unbias = 1 / sqrt(1 - beta2^t), the powers by
 // squaring in 64 bits (1 - beta^t loses what 32 hold while it is near zero):
 // beta1's in even lanes, beta2's in odd ones.
-__device__ __forceinline__ void bias(const Scalars& s, uint32_t t, Common& k) {
-  const bool odd = threadIdx.x & 1;
-  double x = odd ? s.beta2 : s.beta1, power = 1.0;
-  for (; t != 0; t >>= 1) {
-    if (t & 1) power *= x;
-    x *= x;
-  }
-  const float rest = (float)(1.0 - power);
-  const float out = odd ? 1.f / sqrtf(rest) : s.lr / rest;
-  k.rate = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(out), 0));
-  k.unbias =
-      __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(out), 1));
-}
-
-// Step counts are read by all workgroups and written once, by the first wave of
-// the last workgroup that has read them. (A launch of its own for that took 3 to
-// 4 us a step; this takes 0.6.) One address takes an arrival in 12 ns, so they
-// arrive at 32, and the last of each of these at one. Counters wrap by
-// themselves to the zero that the next launch needs.
-__device__ __forceinline__ bool last_to_arrive(unsigned* tickets) {
-  __syncthreads();  // all four waves have read
-  bool last = false;
-  if (threadIdx.x == 0) {
-    const unsigned groups = gridDim.x, line = blockIdx.x % kTicketLines;
-    const unsigned lines = groups < kTicketLines ? groups : kTicketLines;
-    const unsigned of_line = (groups - line + kTicketLines - 1) / kTicketLines;
-    if (atomicInc(tickets + 32 * (1 + line), of_line - 1) == of_line - 1)
-      last = atomicInc(tickets, lines - 1) == lines - 1;
-  }
-  return threadIdx.x < 64 && __builtin_amdgcn_readfirstlane(last);
-}
-
-template <int Bits>
-__global__ __launch_bounds__(kBlock) void update_kernel(
-    const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
-    long nchunks, int first, int count, int* steps, unsigned* tickets,
-    const Grads grads, const Scalars s) {
-  // A launch without chunks has one workgroup that counts.
-  const bool some = blockIdx.x < nchunks;
-  const Chunk chunk = some ? chunks[blockIdx.x] : Chunk{first, 0};
-  const int at = chunk.tensor - first;
-  const void* const grad = grads.g[at];
-  const int step = __hip_atomic_load(steps + chunk.tensor, __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_AGENT) + 1;
-  if (last_to_arrive(tickets)) {
-    for (int i = threadIdx.x; i < count; i += 64)
-      if (grads.g[i] != nullptr) steps[first + i] += 1;
-  }
-  if (!some || grad == nullptr) return;
-  const Tensor t = tensors[chunk.tensor];
+__device__ __forceinline__ Common common(const Scalars& s, uint32_t key,
+                                         uint32_t t) {
   Common k;
   k.clip = 1.f;
   if (s.norm != nullptr) {
@@ -359,23 +260,186 @@ __global__ __launch_bounds__(kBlock) void update_kernel(
   k.rest2 = s.rest2;
   k.eps = s.eps;
   k.keep = s.keep;
-  bias(s, (uint32_t)step, k);
-  k.key = Bits == 8 ? mix(t.key + (uint32_t)step) : 0;
-  const long start = (long)chunk.index * kChunk;
-  const uint32_t gt = (grads.types[at / 16] >> (2 * (at % 16))) & 3;
-  switch (t.type * 4 + gt) {
-    case kF32 * 4 + kF32:
-      return update_tensor<Bits, float, float>(t, grad, start, k);
-    case kF32 * 4 + kBF16:
-      return update_tensor<Bits, float, __hip_bfloat16>(t, grad, start, k);
-    case kF32 * 4 + kF16:
-      return update_tensor<Bits, float, __half>(t, grad, start, k);
-    case kBF16 * 4 + kBF16:
-      return update_tensor<Bits, __hip_bfloat16, __hip_bfloat16>(t, grad, start,
-                                                                 k);
-    case kF16 * 4 + kF16:
-      return update_tensor<Bits, __half, __half>(t, grad, start, k);
+  k.key = mix(key + t);
+  const bool odd = threadIdx.x & 1;
+  double x = odd ? s.beta2 : s.beta1, power = 1.0;
+  for (; t != 0; t >>= 1) {
+    if (t & 1) power *= x;
+    x *= x;
   }
+  const float rest = (float)(1.0 - power);
+  const float out = odd ? 1.f / sqrtf(rest) : s.lr / rest;
+  k.rate = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(out), 0));
+  k.unbias =
+      __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(out), 1));
+  return k;
+}
+
+// Step counts are read by all workgroups and written once, by the first wave of
+// the last workgroup that has read them. (A launch of its own for that took 3 to
+// 4 us a step.) One address takes an arrival in 12 ns, so they arrive at 32, and
+// the last of each of these at one. Counters wrap by themselves to the zero that
+// the next launch needs.
+__device__ __forceinline__ unsigned on_line() {  // workgroups of this one's line
+  return (gridDim.x - blockIdx.x % kTicketLines + kTicketLines - 1) /
+         kTicketLines;
+}
+
+__device__ __forceinline__ unsigned arrive(unsigned* tickets) {
+  return atomicInc(tickets + 32 * (1 + blockIdx.x % kTicketLines),
+                   on_line() - 1);
+}
+
+// Whether this workgroup, given what arrive() returned, was the last.
+__device__ __forceinline__ bool last(unsigned* tickets, unsigned arrived) {
+  if (arrived != on_line() - 1) return false;
+  const unsigned lines = gridDim.x < kTicketLines ? gridDim.x : kTicketLines;
+  return atomicInc(tickets, lines - 1) == lines - 1;
+}
+
+template <int Bits, typename P, typename G, bool Full>
+__device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
+                                             const int* steps,
+                                             unsigned* tickets,
+                                             unsigned& arrived,
+                                             const Scalars& s) {
+  typedef typename P::Elem PElem;
+  typedef typename G::Elem GElem;
+  const Global<PElem> param = (Global<PElem>)w.p;
+  const Global<const GElem> g_at = (Global<const GElem>)grad + w.start;
+  const Global<float> m32 = (Global<float>)w.m, v32 = (Global<float>)w.r;
+  const Global<uint8_t> m8 = (Global<uint8_t>)w.m, r8 = (Global<uint8_t>)w.r;
+  const Global<uint8_t> m8s = (Global<uint8_t>)w.ms;
+  const Global<uint8_t> r8s = (Global<uint8_t>)w.rs;
+  const int n = w.left;
+
+  // All loads first: they are on their way while the step is counted.
+  typename P::Quad pq[kQuads];
+  typename G::Quad gq[kQuads];
+  f32x4 mq[kQuads], vq[kQuads];
+  uint32_t mw[kQuads], rw[kQuads], ms[kQuads], rs[kQuads];
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    const int i = 4 * (q * kBlock + (int)threadIdx.x);
+    if constexpr (Bits == 32) {
+      mq[q] = load4<Full, F32>(m32, i, n);
+      vq[q] = load4<Full, F32>(v32, i, n);
+    } else {
+      mw[q] = load_codes<Full>(m8, i, n);
+      rw[q] = load_codes<Full>(r8, i, n);
+      ms[q] = Full || i < n ? m8s[i / kGroup] : 0;
+      rs[q] = Full || i < n ? r8s[i / kGroup] : 0;
+    }
+    gq[q] = load4<Full, G>(g_at, i, n);
+    pq[q] = load4<Full, P>(param, i, n);
+  }
+  const int step = __hip_atomic_load(steps + w.tensor, __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT) + 1;
+  __syncthreads();  // all four waves have read it
+  if (threadIdx.x == 0) arrived = arrive(tickets);
+  const Common k = common(s, w.key, (uint32_t)step);
+
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    const int i = 4 * (q * kBlock + (int)threadIdx.x);
+    float p[4], g[4], m[4], v[4], root[4];
+    widen<P>(pq[q], p);
+    widen<G>(gq[q], g);
+    if constexpr (Bits == 32) {
+      widen<F32>(mq[q], m);
+      widen<F32>(vq[q], v);
+      moments(k, g, m, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
+      store4<Full, F32>(m32, i, n, m);
+      store4<Full, F32>(v32, i, n, v);
+    } else {
+      decode(mw[q], pow2(ms[q]), m);
+      decode(rw[q], pow2(rs[q]), root);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = root[c] * root[c];
+      moments(k, g, m, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
+
+      // All eight lanes of a group come here, also those behind the end.
+      const uint32_t em = max8(top_bits(m)) >> 23;
+      const uint32_t ev = max8(top_bits(v)) >> 23;
+      const uint32_t sm = em < 14 ? 7 : em - 7;
+      const uint32_t sr = (uint32_t)(((int)ev - 127) >> 1) + 120;
+      const float im = pow2(254 - sm), ir = pow2(254 - sr);
+      const long at = w.start + i;
+      const uint32_t key = k.key + 0x9E3779B9u * (uint32_t)(at >> 32);
+      float zm[4], zr[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t h = mix((uint32_t)(at + c) ^ key);
+        zm[c] = round_by_chance(m[c], im, h & 0xFFFFu, 0.f);
+        zr[c] = round_by_chance(root[c], ir, h >> 16, 1.f);
+      }
+      store_codes<Full>(m8, i, n, encode(zm));
+      store_codes<Full>(r8, i, n, encode(zr));
+      if ((Full || i < n) && threadIdx.x % (kGroup / 4) == 0) {
+        m8s[i / kGroup] = (uint8_t)sm;
+        r8s[i / kGroup] = (uint8_t)sr;
+      }
+    }
+    move(k, m, root, p);
+    store4<Full, P>(param, i, n, p);
+  }
+}
+
+template <int Bits, typename P, typename G>
+__device__ __forceinline__ void update_tensor(const Work& w, const void* grad,
+                                              const int* steps,
+                                              unsigned* tickets,
+                                              unsigned& arrived,
+                                              const Scalars& s) {
+  if (w.left == kChunk)
+    update_chunk<Bits, P, G, true>(w, grad, steps, tickets, arrived, s);
+  else
+    update_chunk<Bits, P, G, false>(w, grad, steps, tickets, arrived, s);
+}
+
+template <int Bits>
+__global__ __launch_bounds__(kBlock) void update_kernel(
+    const Work* __restrict__ work, long nwork, int first, int count, int* steps,
+    unsigned* tickets, const Grads grads, const Scalars s) {
+  unsigned arrived = 0;
+  const void* grad = nullptr;
+  Work w;
+  if (blockIdx.x < nwork) {  // without work, one workgroup counts
+    w = work[blockIdx.x];
+    grad = grads.g[w.tensor - first];
+  }
+  if (grad == nullptr) {
+    if (threadIdx.x == 0) arrived = arrive(tickets);
+  } else {
+    const int at = w.tensor - first;
+    const uint32_t type = (grads.types[at / 16] >> (2 * (at % 16))) & 3;
+    switch (w.type * 4 + type) {
+      case kF32 * 4 + kF32:
+        update_tensor<Bits, F32, F32>(w, grad, steps, tickets, arrived, s);
+        break;
+      case kF32 * 4 + kBF16:
+        update_tensor<Bits, F32, BF16>(w, grad, steps, tickets, arrived, s);
+        break;
+      case kF32 * 4 + kF16:
+        update_tensor<Bits, F32, F16>(w, grad, steps, tickets, arrived, s);
+        break;
+      case kBF16 * 4 + kBF16:
+        update_tensor<Bits, BF16, BF16>(w, grad, steps, tickets, arrived, s);
+        break;
+      case kF16 * 4 + kF16:
+        update_tensor<Bits, F16, F16>(w, grad, steps, tickets, arrived, s);
+        break;
+    }
+  }
+  if (threadIdx.x >= 64) return;
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x == 0 &&
+                                     last(tickets, arrived)))
+    for (int i = threadIdx.x; i < count; i += 64)
+      if (grads.g[i] != nullptr) steps[first + i] += 1;
 }
 
 // ---------------------------------------------------------------------------
@@ -385,22 +449,25 @@ __global__ __launch_bounds__(kBlock) void update_kernel(
 // spans alone, so the result is the same every time.
 
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const T* base, long begin,
+__device__ __forceinline__ double chunk_squares(const void* ptr, int chunk,
                                                 long n) {
-  constexpr int kElems = kNormChunkBytes / sizeof(T);
+  constexpr int kElems = kNormChunkBytes / sizeof(typename T::Elem);
+  const Global<const typename T::Elem> base =
+      (Global<const typename T::Elem>)ptr + (long)chunk * kElems;
+  n -= (long)chunk * kElems;
   double sum[4] = {0, 0, 0, 0};
-  if (begin + kElems <= n) {
+  if (n >= kElems) {
 #pragma unroll
     for (int q = 0; q < kElems / (4 * kBlock); ++q) {
       float x[4];
-      load4<true>(base, begin + 4 * ((long)q * kBlock + threadIdx.x), n, x);
+      widen<T>(load4<true, T>(base, 4 * (q * kBlock + (int)threadIdx.x), 0), x);
 #pragma unroll
       for (int c = 0; c < 4; ++c) sum[c] = fma((double)x[c], (double)x[c], sum[c]);
     }
   } else {
-    for (long i = begin + 4 * threadIdx.x; i < n; i += 4 * kBlock) {
+    for (int i = 4 * threadIdx.x; i < (int)n; i += 4 * kBlock) {
       float x[4];
-      load4<false>(base, i, n, x);
+      widen<T>(load4<false, T>(base, i, (int)n), x);
 #pragma unroll
       for (int c = 0; c < 4; ++c) sum[c] = fma((double)x[c], (double)x[c], sum[c]);
     }
@@ -427,18 +494,16 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(const Spans spans,
   int span = 0;
   for (int c = blockIdx.x; c < spans.start[spans.count]; c += gridDim.x) {
     while (c >= spans.start[span + 1]) ++span;
-    const long bytes = (long)(c - spans.start[span]) * kNormChunkBytes;
-    const void* const ptr = spans.ptr[span];
-    const long n = spans.n[span];
+    const int chunk = c - spans.start[span];
     switch (spans.type[span]) {
       case kF32:
-        sum += chunk_squares((const float*)ptr, bytes / 4, n);
+        sum += chunk_squares<F32>(spans.ptr[span], chunk, spans.n[span]);
         break;
       case kBF16:
-        sum += chunk_squares((const __hip_bfloat16*)ptr, bytes / 2, n);
+        sum += chunk_squares<BF16>(spans.ptr[span], chunk, spans.n[span]);
         break;
       case kF16:
-        sum += chunk_squares((const __half*)ptr, bytes / 2, n);
+        sum += chunk_squares<F16>(spans.ptr[span], chunk, spans.n[span]);
         break;
     }
   }
@@ -458,9 +523,9 @@ __global__ __launch_bounds__(kBlock) void norm_finish_kernel(
 
 bool supported(int p, int g) { return p == g || p == kF32; }
 
-void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
-            int first, int count, int* steps, unsigned* tickets,
-            const Grads& grads, const Hyper& h, hipStream_t stream) {
+void update(int bits, const Work* work, long nwork, int first, int count,
+            int* steps, unsigned* tickets, const Grads& grads, const Hyper& h,
+            hipStream_t stream) {
   const Scalars s = {h.beta1,
                      h.beta2,
                      (float)h.lr,
@@ -470,13 +535,13 @@ void update(int bits, const Tensor* tensors, const Chunk* chunks, long nchunks,
                      (float)(1.0 - h.lr * h.weight_decay),
                      (float)h.max_norm,
                      h.norm};
-  const dim3 grid((unsigned)(nchunks > 0 ? nchunks : 1));
+  const dim3 grid((unsigned)(nwork > 0 ? nwork : 1));
   if (bits == 8)
     update_kernel<8><<<grid, kBlock, 0, stream>>>(
-        tensors, chunks, nchunks, first, count, steps, tickets, grads, s);
+        work, nwork, first, count, steps, tickets, grads, s);
   else
     update_kernel<32><<<grid, kBlock, 0, stream>>>(
-        tensors, chunks, nchunks, first, count, steps, tickets, grads, s);
+        work, nwork, first, count, steps, tickets, grads, s);
 }
 
 int norm_blocks(const Spans& spans) {

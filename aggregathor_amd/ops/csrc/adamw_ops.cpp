@@ -158,19 +158,17 @@ class Plan {
     const auto stream = current.stream();
     if (capturing()) {
       if (!captured_)
-        for (const Tensor& t : {device_table_, device_chunks_, tickets_})
+        for (const Tensor& t : {device_work_, tickets_})
           captured_tables().push_back(t);
       captured_ = true;
     } else if (current != laid_out_on_) {
       // The allocator must not give these to others before this step is done.
-      for (const Tensor& t : {device_table_, device_chunks_, tickets_})
+      for (const Tensor& t : {device_work_, tickets_})
         t.record_stream(
             c10::hip::HIPStreamMasqueradingAsCUDA(current).unwrap());
     }
-    const auto* tensors =
-        reinterpret_cast<const adamw::Tensor*>(device_table_.data_ptr());
-    const auto* chunks =
-        reinterpret_cast<const adamw::Chunk*>(device_chunks_.data_ptr());
+    const auto* work =
+        reinterpret_cast<const adamw::Work*>(device_work_.data_ptr());
     auto* tickets = reinterpret_cast<unsigned*>(tickets_.data_ptr());
     int* steps = steps_.data_ptr<int>();
     for (size_t first = 0; first < count; first += adamw::kMaxTensors) {
@@ -182,13 +180,13 @@ class Plan {
         const size_t k = i - first;
         any = true;
         // A tensor of no elements has a gradient all the same: any address.
-        g.g[k] = held[i].numel() > 0 ? held[i].data_ptr() : (const void*)tensors;
+        g.g[k] = held[i].numel() > 0 ? held[i].data_ptr() : (const void*)work;
         g.types[k / 16] |= (uint32_t)types[i] << (2 * (k % 16));
       }
       if (!any) continue;
-      const int64_t begin = chunk_start_[first];
-      adamw::update(bits_, tensors, chunks + begin, chunk_start_[last] - begin,
-                    (int)first, (int)(last - first), steps,
+      const int64_t begin = work_start_[first];
+      adamw::update(bits_, work + begin, work_start_[last] - begin, (int)first,
+                    (int)(last - first), steps,
                     tickets + first / adamw::kMaxTensors * adamw::kTicketInts,
                     g, hyper, stream);
       C10_HIP_CHECK(hipGetLastError());
@@ -209,7 +207,7 @@ class Plan {
     for (size_t i = 0; i < params_.size(); ++i) {
       const auto& t = table_[i];
       if (params_[i].data_ptr() != t.p || m_[i].data_ptr() != t.m ||
-          r_[i].data_ptr() != t.r || params_[i].numel() != t.n ||
+          r_[i].data_ptr() != t.r || params_[i].numel() != numel_[i] ||
           params_[i].device() != steps_.device() ||
           dtype_of(params_[i], "adamw: parameter") != t.type ||
           !same_layout(params_[i], m_[i]) || !same_layout(params_[i], r_[i]))
@@ -217,7 +215,7 @@ class Plan {
       if (bits_ == 8 &&
           (ms_[i].data_ptr() != t.ms || rs_[i].data_ptr() != t.rs ||
            ms_[i].numel() != rs_[i].numel() ||
-           ms_[i].numel() != (t.n + adamw::kGroup - 1) / adamw::kGroup))
+           ms_[i].numel() != (numel_[i] + adamw::kGroup - 1) / adamw::kGroup))
         return true;
     }
     return false;
@@ -251,9 +249,8 @@ class Plan {
                 "each parameter, on their device");
     const auto state_type =
         bits_ == 8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
-    std::vector<adamw::Tensor> table(count);
-    std::vector<adamw::Chunk> chunks;
-    std::vector<int64_t> chunk_start(count + 1, 0);
+    std::vector<adamw::Work> table(count), work;
+    std::vector<int64_t> work_start(count + 1, 0);
     std::vector<Range> written{range_of(steps_)};
     for (size_t i = 0; i < count; ++i) {
       const Tensor& p = params_[i];
@@ -269,10 +266,10 @@ class Plan {
                   bits_ == 8 ? "exp_avg_root" : "exp_avg_sq", i);
       const int64_t n = p.numel();
       auto& t = table[i];
+      t.tensor = (int)i;
       t.p = p.data_ptr();
       t.m = m_[i].data_ptr();
       t.r = r_[i].data_ptr();
-      t.n = n;
       t.key = mix(seed_ + 0x9E3779B9u * (uint32_t)(i + 1));
       t.type = dtype_of(p, "adamw: parameter");
       written.push_back(range_of(p));
@@ -292,11 +289,22 @@ class Plan {
         t.ms = reinterpret_cast<uint8_t*>(ms_[i].data_ptr());
         t.rs = reinterpret_cast<uint8_t*>(rs_[i].data_ptr());
       }
-      const int64_t parts = (n + adamw::kChunk - 1) / adamw::kChunk;
-      TORCH_CHECK(parts <= INT32_MAX, "adamw: parameter ", i, " is too large");
-      for (int64_t c = 0; c < parts; ++c)
-        chunks.push_back({(int)i, (int)c});
-      chunk_start[i + 1] = chunk_start[i] + parts;
+      for (int64_t start = 0; start < n; start += adamw::kChunk) {
+        adamw::Work w = t;
+        const int64_t state = start * (bits_ / 8);
+        w.p = (char*)t.p + start * p.element_size();
+        w.m = (char*)t.m + state;
+        w.r = (char*)t.r + state;
+        if (bits_ == 8) {
+          w.ms = t.ms + start / adamw::kGroup;
+          w.rs = t.rs + start / adamw::kGroup;
+        }
+        w.start = start;
+        w.left = (int)std::min<int64_t>(n - start, adamw::kChunk);
+        work.push_back(w);
+      }
+      TORCH_CHECK(work.size() <= INT32_MAX, "adamw: too many elements");
+      work_start[i + 1] = (int64_t)work.size();
     }
     std::sort(written.begin(), written.end(),
               [](const Range& a, const Range& b) { return a.lo < b.lo; });
@@ -312,14 +320,15 @@ class Plan {
     tickets_ = torch::zeros(
         {launches * adamw::kTicketInts},
         torch::TensorOptions().device(device).dtype(torch::kInt32));
-    // Uploads wait for the stream, so another one may use all of these next.
-    device_table_ = upload(table, device);
-    if (chunks.empty()) chunks.push_back({0, 0});
-    device_chunks_ = upload(chunks, device);
+    // The upload waits for the stream, so another may use all of these next.
+    if (work.empty()) work.push_back(table[0]);
+    device_work_ = upload(work, device);
     laid_out_on_ = c10::hip::getCurrentHIPStream();
     steps_at_ = steps_.data_ptr();
+    numel_.clear();
+    for (const Tensor& p : params_) numel_.push_back(p.numel());
     table_ = std::move(table);
-    chunk_start_ = std::move(chunk_start);
+    work_start_ = std::move(work_start);
     written_ = std::move(written);
     captured_ = false;
   }
@@ -339,10 +348,11 @@ class Plan {
   std::vector<Tensor> params_, m_, ms_, r_, rs_;
   Tensor steps_;
   uint32_t seed_;
-  std::vector<adamw::Tensor> table_;
-  std::vector<int64_t> chunk_start_;
+  std::vector<adamw::Work> table_;  // each tensor's first
+  std::vector<int64_t> work_start_;  // before each tensor's, in device_work_
+  std::vector<int64_t> numel_;
   std::vector<Range> written_;
-  Tensor device_table_, device_chunks_, tickets_;
+  Tensor device_work_, tickets_;
   c10::hip::HIPStream laid_out_on_ = c10::hip::getDefaultHIPStream();
   const void* steps_at_ = nullptr;
   bool captured_ = false;
