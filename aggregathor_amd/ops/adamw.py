@@ -137,7 +137,7 @@ def adamw_step(plan, grads, lr, beta1=0.9, beta2=0.999, eps=1e-8,
             ("lr", lr, 0. <= lr < math.inf),
             ("beta1", beta1, 0. <= beta1 < 1.),
             ("beta2", beta2, 0. <= beta2 < 1.),
-            ("eps", eps, 1.2e-38 <= eps < 3e38),
+            ("eps", eps, 1.2e-38 <= eps <= 1e30),
             ("weight_decay", weight_decay, 0. <= weight_decay < math.inf)):
         if not ok:
             raise RuntimeError(f"adamw: {name} = {value} is out of range")

@@ -2,7 +2,8 @@
 the CPU path, and what the HIP kernels are compared with.
 
 States are computed in the kernels' order, one rounding an operation, so that
-8-bit codes come out the same bit by bit.
+they come out the same bit by bit, but for codes of a root where the kernels'
+square root is off in its last bit and the rounding is next to a border.
 """
 
 import torch
@@ -80,16 +81,18 @@ def _largest(x):
 
 
 def round_by_chance(x, exponents, chance, least):
-    """Codes of x: rounded up with a probability of ``chance / 2**16`` (a
-    constant 2**15 rounds to nearest)."""
+    """Codes of x, ``floor(|x| / scale / quantum + chance / 2**16)`` quanta: up
+    with that probability (a constant 2**15 rounds to nearest)."""
     n = x.numel()
     inv = torch.exp2(127. - exponents.float())
     y = (_grouped(x.abs()) * inv[:, None]).view(-1)[:n]
-    quantum = torch.exp2(((y.view(torch.int32) >> 23) - 127).clamp(
-        -6, 127).float() - 3.)
-    count = torch.floor(y / quantum + chance * 2. ** -16)
-    count = torch.where(y > 0, count.clamp(min=least), count)
-    z = torch.copysign(count * quantum, x)
+    # The chance goes right below the last bit that stays; below 2^-6, where
+    # the quantum stays 2^-9, as if y had 2^-6 to it.
+    low = torch.where(y < 2. ** -6, 2. ** -6, 0.)
+    bits = ((y + low).view(torch.int32) + (chance.int() << 4)) & -0x100000
+    z = bits.view(torch.float32) - low
+    z = torch.where(y > 0, z.clamp(min=least * 2. ** -9), z)
+    z = torch.copysign(z, x)
     z = torch.where(y.isfinite(), z, torch.full_like(z, float("nan")))
     return z.to(torch.float8_e4m3fn)
 

@@ -22,9 +22,13 @@
 // its inputs, the same on every rank and in every replay.
 // The step itself uses the new m and v before they are rounded.
 //
-// The arithmetic on m, v and their codes is plain IEEE fp32, one rounding an
-// operation (no contraction into fused multiply-adds), so that states can be
-// compared with another implementation's bit by bit.
+// m, v and the scales are plain IEEE fp32, one rounding an operation (no
+// contraction into fused multiply-adds), so they can be compared with another
+// implementation's bit by bit. The root and the quotient take the hardware's
+// square root and reciprocal, which are off by a unit in the last place at most
+// (seen over all normal numbers): the full sequences for the last half bit are
+// 25 instructions an element, and with 8-bit states the vector units were as
+// busy as the memory (114 instructions an element for 16 bytes).
 
 #include <hip/hip_runtime.h>
 
@@ -143,6 +147,12 @@ __device__ __forceinline__ void store_codes(Global<uint8_t> base, int i, int n,
   }
 }
 
+// What all elements of a workgroup share.
+struct Common {
+  float clip, beta1, rest1, beta2, rest2, eps, keep, rate, unbias;
+  uint32_t key;
+};
+
 // ---------------------------------------------------------------------------
 // 8-bit states
 
@@ -174,18 +184,15 @@ __device__ __forceinline__ float pow2(uint32_t biased) {
   return __uint_as_float(biased << 23);
 }
 
-// x times inv (a power of two, 1 / the group's scale), rounded to a value that
-// e4m3 has: up with the probability of chance / 2^16. What is not finite
-// becomes a NaN, since the format has no infinity.
-__device__ __forceinline__ float round_by_chance(float x, float inv,
-                                                 uint32_t chance, float least) {
-  const float y = fabsf(x) * inv;
-  uint32_t e = __float_as_uint(y) >> 23;
-  e = e < 121 ? 121 : e;  // below 2^-6 the quantum stays 2^-9
-  float t = floorf(y * pow2(257 - e) + (float)chance * 0x1p-16f);
-  if (y > 0.f) t = fmaxf(t, least);
-  const float z = copysignf(t * pow2(e - 3), x);
-  return y < INFINITY ? z : NAN;
+// y >= 0 rounded to a value that e4m3 has, up with a probability of chance / 2^16:
+// floor(y / quantum + chance / 2^16) quanta. Above 2^-6 the quantum is the value
+// of the lowest of the three leading bits of the mantissa, so adding the chance
+// right below that bit and cutting off there does it. Below, the quantum stays
+// 2^-9, as if y had 2^-6 to it.
+__device__ __forceinline__ float round_by_chance(float y, uint32_t chance) {
+  const float low = y < 0x1p-6f ? 0x1p-6f : 0.f;
+  const uint32_t bits = __float_as_uint(y + low) + (chance << 4);
+  return __uint_as_float(bits & 0xFFF00000u) - low;
 }
 
 // Largest of a value over the eight lanes that share a group.
@@ -199,26 +206,70 @@ __device__ __forceinline__ uint32_t max8(uint32_t v) {
   return v > o ? v : o;
 }
 
-// Bits of the largest |x| that is finite; as whole numbers they order alike.
+// Bits of the largest |x|; as whole numbers they order alike, with infinity and
+// NaN above all others.
+constexpr uint32_t kInf = 0x7F800000u;
+
+template <bool Finite>
 __device__ __forceinline__ uint32_t top_bits(const float (&x)[4]) {
   uint32_t top = 0;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     uint32_t b = __float_as_uint(x[c]) & 0x7FFFFFFFu;
-    b = b < 0x7F800000u ? b : 0u;
+    if (Finite) b = b < kInf ? b : 0u;
     top = top > b ? top : b;
   }
   return top;
 }
 
+// One quad's new 8-bit states.
+struct Codes {
+  uint32_t m, r, m_scale, r_scale;
+};
+
+// From m and v; gives the denominators too. `tm` and `tv` are top_bits of the
+// group. Plain: everything in the wave is finite.
+template <bool Plain>
+__device__ __forceinline__ Codes encode_states(const Common& k, long at,
+                                               uint32_t tm, uint32_t tv,
+                                               const float (&m)[4],
+                                               const float (&v)[4],
+                                               float (&denominator)[4]) {
+  Codes out;
+  const uint32_t em = tm >> 23;
+  out.m_scale = em < 14 ? 7 : em - 7;
+  const int half = ((int)(tv >> 23) - 127) >> 1;
+  out.r_scale = (uint32_t)(half + 120);
+  const float im = pow2(254 - out.m_scale);
+  const float root_unit = pow2(out.r_scale) * k.unbias;
+  const uint32_t key = k.key + 0x9E3779B9u * (uint32_t)(at >> 32);
+  float zm[4], zr[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t h = mix((uint32_t)(at + c) ^ key);
+    zm[c] = copysignf(round_by_chance(fabsf(m[c]) * im, h & 0xFFFFu), m[c]);
+    // v / scale^2 first: the hardware's root takes denormals for zero. What is
+    // still one is 2^71 below the group's largest root, and raised to that.
+    const float y = __builtin_amdgcn_sqrtf(
+        fmaxf(ldexpf(v[c], 2 * (7 - half)), 0x1p-126f));
+    denominator[c] = __builtin_fmaf(y, root_unit, k.eps);
+    zr[c] = fmaxf(round_by_chance(y, h >> 16), v[c] > 0.f ? 0x1p-9f : 0.f);
+    if (!Plain) {
+      // NaN where there is none to store (the format has no infinity), and the
+      // formula's own values in the denominator.
+      const bool fine_m = fabsf(m[c]) < INFINITY, fine_v = v[c] < INFINITY;
+      zm[c] = fine_m ? zm[c] : NAN;
+      zr[c] = fine_v ? zr[c] : NAN;
+      denominator[c] = fine_v ? denominator[c] : v[c];
+    }
+  }
+  out.m = encode(zm);
+  out.r = encode(zr);
+  return out;
+}
+
 // ---------------------------------------------------------------------------
 // The update
-
-// What all elements of a workgroup share.
-struct Common {
-  float clip, beta1, rest1, beta2, rest2, eps, keep, rate, unbias;
-  uint32_t key;
-};
 
 __device__ __forceinline__ void moments(const Common& k, const float (&g)[4],
                                         float (&m)[4], float (&v)[4]) {
@@ -231,10 +282,20 @@ __device__ __forceinline__ void moments(const Common& k, const float (&g)[4],
 }
 
 __device__ __forceinline__ void move(const Common& k, const float (&m)[4],
-                                     const float (&root)[4], float (&p)[4]) {
+                                     const float (&denominator)[4],
+                                     float (&p)[4]) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    p[c] = p[c] * k.keep - k.rate * (m[c] / (root[c] * k.unbias + k.eps));
+    p[c] = p[c] * k.keep -
+           k.rate * (m[c] * __builtin_amdgcn_rcpf(denominator[c]));
+}
+
+// The hardware's root, which takes denormals for zero, of a number that may be
+// one.
+__device__ __forceinline__ float root_of(float v) {
+  const bool low = v < 0x1p-96f;
+  return __builtin_amdgcn_sqrtf(v * (low ? 0x1p64f : 1.f)) *
+         (low ? 0x1p-32f : 1.f);
 }
 
 struct Scalars {
@@ -342,49 +403,42 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
 #pragma unroll
   for (int q = 0; q < kQuads; ++q) {
     const int i = 4 * (q * kBlock + (int)threadIdx.x);
-    float p[4], g[4], m[4], v[4], root[4];
+    float p[4], g[4], m[4], v[4], denominator[4];
     widen<P>(pq[q], p);
     widen<G>(gq[q], g);
     if constexpr (Bits == 32) {
       widen<F32>(mq[q], m);
       widen<F32>(vq[q], v);
       moments(k, g, m, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
       store4<Full, F32>(m32, i, n, m);
       store4<Full, F32>(v32, i, n, v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        denominator[c] = root_of(v[c]) * k.unbias + k.eps;
     } else {
       decode(mw[q], pow2(ms[q]), m);
-      decode(rw[q], pow2(rs[q]), root);
+      decode(rw[q], pow2(rs[q]), v);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = root[c] * root[c];
+      for (int c = 0; c < 4; ++c) v[c] = v[c] * v[c];
       moments(k, g, m, v);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) root[c] = sqrtf(v[c]);
-
       // All eight lanes of a group come here, also those behind the end.
-      const uint32_t em = max8(top_bits(m)) >> 23;
-      const uint32_t ev = max8(top_bits(v)) >> 23;
-      const uint32_t sm = em < 14 ? 7 : em - 7;
-      const uint32_t sr = (uint32_t)(((int)ev - 127) >> 1) + 120;
-      const float im = pow2(254 - sm), ir = pow2(254 - sr);
-      const long at = w.start + i;
-      const uint32_t key = k.key + 0x9E3779B9u * (uint32_t)(at >> 32);
-      float zm[4], zr[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t h = mix((uint32_t)(at + c) ^ key);
-        zm[c] = round_by_chance(m[c], im, h & 0xFFFFu, 0.f);
-        zr[c] = round_by_chance(root[c], ir, h >> 16, 1.f);
+      uint32_t tm = max8(top_bits<false>(m)), tv = max8(top_bits<false>(v));
+      Codes codes;
+      if (__builtin_expect(__any(tm >= kInf || tv >= kInf), 0)) {
+        tm = max8(top_bits<true>(m));
+        tv = max8(top_bits<true>(v));
+        codes = encode_states<false>(k, w.start + i, tm, tv, m, v, denominator);
+      } else {
+        codes = encode_states<true>(k, w.start + i, tm, tv, m, v, denominator);
       }
-      store_codes<Full>(m8, i, n, encode(zm));
-      store_codes<Full>(r8, i, n, encode(zr));
+      store_codes<Full>(m8, i, n, codes.m);
+      store_codes<Full>(r8, i, n, codes.r);
       if ((Full || i < n) && threadIdx.x % (kGroup / 4) == 0) {
-        m8s[i / kGroup] = (uint8_t)sm;
-        r8s[i / kGroup] = (uint8_t)sr;
+        m8s[i / kGroup] = (uint8_t)codes.m_scale;
+        r8s[i / kGroup] = (uint8_t)codes.r_scale;
       }
     }
-    move(k, m, root, p);
+    move(k, m, denominator, p);
     store4<Full, P>(param, i, n, p);
   }
 }

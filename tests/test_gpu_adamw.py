@@ -70,6 +70,24 @@ def _equal(a, b):
         a.nan_to_num(7.), b.nan_to_num(7.))
 
 
+def _check_states(a, b, what=""):
+    """8-bit states of the kernel (a) against the plain form's (b): m's codes
+    and all scales bit by bit. The kernel's square root may be off by a unit in
+    the last place, 2^-23 of it, and so y / quantum + u, which is below 17, by
+    at most 17 2^-23 < 2^-18. Where that has a whole number within it, the root's
+    code may be its neighbour: with a chance of 2^-17 for each element, so that
+    more than 8 + 4 n 2^-17 are not to be expected."""
+    (am, ams, ar, ars), (bm, bms, br, brs) = a, b
+    assert _equal(am, bm) and _equal(ams, bms) and _equal(ars, brs), what
+    x, y = (t.detach().cpu().contiguous().view(torch.uint8).int().reshape(-1)
+            for t in (ar, br))
+    x, y = (torch.where(t & 127 == 127, 127, t) for t in (x, y))  # either NaN
+    off = (x - y).abs()
+    n = off.numel()
+    assert n == 0 or (int(off.max()) <= 1
+                      and int((off > 0).sum()) <= 8 + 4 * n / 2 ** 17), what
+
+
 # ---------------------------------------------------------------------------- #
 # Norm
 
@@ -173,8 +191,7 @@ def test_step8(p_dtype, g_dtype, max_norm):
         what = f"of {SIZES[i]}"
         oracle.check(p[i], x[0], oracle.rounded(bounds[0], x[0], p_dtype),
                      "p " + what)
-        for a, b in zip(own, state):
-            assert _equal(a[i], b[i]), what
+        _check_states([c[i] for c in own], [c[i] for c in state], what)
         m, ms, r, rs = (column[i] for column in own)
         oracle.check8(m, ms, ops.adamw8_values(m, ms), x[1], False, "m " + what)
         oracle.check8(r, rs, ops.adamw8_values(r, rs), x[2].sqrt(), True,
@@ -196,10 +213,12 @@ def test_step8_states_at_odd_starts_leave_their_neighbours():
     ops.adamw_step(ops.adamw8_plan(params, *state,
                                    torch.zeros(3, dtype=torch.int32)),
                    grads, **HYPER)
-    for (_, flat), column in zip(flats, state):
+    whole = []
+    for (_, flat), column, kind in zip(flats, state, kinds):
         want = torch.cat([torch.zeros(3, dtype=torch.uint8)] +
                          [t.view(torch.uint8) for t in column])
-        assert torch.equal(flat.cpu(), want)
+        whole.append((flat.view(kind), want.view(kind)))
+    _check_states([x for x, _ in whole], [x for _, x in whole])
     assert float(pflat[0]) == 0
 
 
@@ -211,6 +230,7 @@ def test_nan_infinity_zero_and_denormals(bits):
     grad[64:96] = 0.
     grad[96:128] = 1e-42
     grad[128:160] = 1e25  # its square overflows
+    grad[160:] = 1e-20    # its square is a denormal number
     out = []
     for device in ("cpu", "cuda"):
         p = torch.ones(n, device=device)
@@ -224,8 +244,10 @@ def test_nan_infinity_zero_and_denormals(bits):
         for _ in range(3):
             ops.adamw_step(plan, [grad.to(device)], lr=1e-3)
         out.append([p, *state])
-    for a, b in zip(out[0][1:], out[1][1:]):
-        assert _equal(a, b)
+    if bits == 8:
+        _check_states(out[1][1:], out[0][1:])
+    else:
+        assert all(_equal(a, b) for a, b in zip(out[0][1:], out[1][1:]))
     a, b = (x[0].cpu() for x in out)
     assert torch.equal(a.isnan(), b.isnan())
     # Three steps of 1e-3, each off by 40 u of itself at most.
@@ -264,8 +286,12 @@ def test_missing_gradients_and_many_tensors(bits):
                    [g if ok else None for g, ok in zip(grads, present)],
                    **HYPER)
     assert steps.tolist() == [int(ok) for ok in present]
-    for a, b in zip(own, state):
-        assert all(_equal(x, y) for x, y in zip(a, b))
+    for i in range(1000):
+        a, b = ([c[i] for c in x] for x in (own, state))
+        if bits == 8:
+            _check_states(a, b)
+        else:
+            assert all(_equal(x, y) for x, y in zip(a, b))
     for x, y in zip(p, params):
         torch.testing.assert_close(x.cpu(), y, rtol=1e-6, atol=1e-6)
 
@@ -294,7 +320,13 @@ def test_layouts(bits):
                 out.append((p, opt.state[p]))
             (a, x), (b, y) = out
             torch.testing.assert_close(a, b.cpu(), rtol=1e-6, atol=1e-6)
-            assert all(_equal(x[k], y[k]) for k in x), name
+            assert _equal(x["step"], y["step"])
+            if bits == 8:
+                _check_states(*([s[k] for k in (
+                    "exp_avg", "exp_avg_scale", "exp_avg_root",
+                    "exp_avg_root_scale")] for s in (y, x)), name)
+            else:
+                assert all(_equal(x[k], y[k]) for k in x), name
 
 
 def test_expanded_and_strided_gradients():
@@ -332,9 +364,11 @@ def test_large_tensor_8():
         exponents = R.exponents_of(R._largest(of), root)
         assert torch.equal(scales[-groups:].cpu().view(torch.uint8),
                            exponents.to(torch.uint8))
-        want = R.round_by_chance(values, exponents, chance.float(),
-                                 float(root))
-        assert _equal(codes[-tail:], want)
+        want = R.round_by_chance(values, exponents, chance, float(root))
+        got = codes[-tail:]
+        _check_states((want, scales, got, scales) if root else
+                      (got, scales, want, scales),
+                      (want, scales, want, scales))
     want, bounds = oracle.step(torch.ones(tail), x, torch.zeros(tail),
                                torch.zeros(tail), 1, **HYPER)
     oracle.check(p[-tail:], want[0], oracle.rounded(
