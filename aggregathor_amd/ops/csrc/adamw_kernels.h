@@ -14,7 +14,7 @@ enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 // Elements that share one scale in an 8-bit state.
 constexpr int kGroup = 32;
 // Elements that one workgroup updates.
-constexpr int kChunk = 4096;
+constexpr int kChunk = 1024;
 // Tensors of one update launch: their gradients' addresses travel in the
 // kernel's arguments, of which there are 4 KiB.
 constexpr int kMaxTensors = 448;
