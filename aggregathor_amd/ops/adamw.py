@@ -40,6 +40,7 @@ import math
 
 import torch
 
+from . import _load_extension, _want_hip
 from . import adamw_reference as reference
 
 #: Elements that share a scale in an 8-bit state.
@@ -48,14 +49,17 @@ GROUP = reference.GROUP
 
 def _ext(tensor):
     """The HIP extension for a GPU tensor, None for the plain forms."""
-    from . import _load_extension, _want_hip
     return _load_extension() if _want_hip(tensor) else None
 
 
 def grad_norm(grads):
-    """L2 norm over all elements of all tensors, as one fp32 number on their
-    device (nothing waits for it). Squares are summed in 64 bits."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    """L2 norm over all elements of a tensor, or of all tensors of a list, as one
+    fp32 number on their device (nothing waits for it). Squares are summed in 64
+    bits, in an order that the tensors' sizes and places alone set."""
+    if isinstance(grads, torch.Tensor):
+        grads = (grads,)
+    elif not isinstance(grads, (list, tuple)):
+        grads = list(grads)
     if not grads:
         raise RuntimeError("grad_norm: expected a tensor")
     ext = _ext(grads[0])
@@ -147,4 +151,6 @@ def adamw_step(plan, grads, lr, beta1=0.9, beta2=0.999, eps=1e-8,
         max_norm = 1.
     elif not 1.2e-38 <= max_norm < 3e38:
         raise RuntimeError(f"adamw: max_norm = {max_norm} is out of range")
+    if not isinstance(grads, (list, tuple)):
+        grads = list(grads)
     plan.step(grads, lr, beta1, beta2, eps, weight_decay, norm, max_norm)

@@ -21,7 +21,7 @@ constexpr int kMaxTensors = 448;
 // Spans of one norm launch, likewise, the workgroups of one such launch at
 // most, and the bytes that one of them reads at a time.
 constexpr int kMaxSpans = 160;
-constexpr int kNormBlocks = 2048;
+constexpr int kNormBlocks = 1024;
 constexpr int kNormChunkBytes = 16384;
 
 // What one workgroup updates: `left` elements of a tensor from the element
@@ -86,8 +86,11 @@ struct Spans {
 // Workgroups, and so partial sums, of a launch over these spans.
 int norm_blocks(const Spans& spans);
 
-// partials[b] = the b-th workgroup's sum of squares.
-void norm_partials(const Spans& spans, double* partials, hipStream_t stream);
+// partials[b] = the b-th workgroup's sum of squares. With tickets (zero before,
+// and again after; not shared with a launch that may run at the same time) the
+// last workgroup to arrive goes on to out = sqrt(sum of partials).
+void norm_partials(const Spans& spans, double* partials, unsigned* tickets,
+                   float* out, hipStream_t stream);
 
 // out = sqrt(sum of partials[0..count)).
 void norm_finish(const double* partials, int count, float* out,

@@ -306,7 +306,9 @@ struct Scalars {
 
 // rate = lr / (1 - beta1^t) and unbias = 1 / sqrt(1 - beta2^t), the powers by
 // squaring in 64 bits (1 - beta^t loses what 32 hold while it is near zero):
-// beta1's in even lanes, beta2's in odd ones.
+// beta1's in even lanes, beta2's in odd ones. Every wave does it for itself:
+// with 8-bit states VGG-16 took 367 us so, and 401 us where three waves waited
+// for one.
 __device__ __forceinline__ Common common(const Scalars& s, uint32_t key,
                                          uint32_t t) {
   Common k;
@@ -394,8 +396,9 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
     gq[q] = load4<Full, G>(g_at, i, n);
     pq[q] = load4<Full, P>(param, i, n);
   }
-  const int step = __hip_atomic_load(steps + w.tensor, __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_AGENT) + 1;
+  const int step = __builtin_amdgcn_readfirstlane(
+      __hip_atomic_load(steps + w.tensor, __ATOMIC_RELAXED,
+                        __HIP_MEMORY_SCOPE_AGENT) + 1);
   __syncthreads();  // all four waves have read it
   if (threadIdx.x == 0) arrived = arrive(tickets);
   const Common k = common(s, w.key, (uint32_t)step);
@@ -532,6 +535,7 @@ __device__ __forceinline__ double chunk_squares(const void* ptr, int chunk,
 // Sum over the workgroup, in thread 0.
 __device__ __forceinline__ double block_sum(double v) {
   __shared__ double part[kBlock / 64];
+  __syncthreads();  // the last call's are read
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
@@ -542,8 +546,16 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
+// With tickets the last workgroup to arrive adds the partial sums up, always in
+// the same order. The sums are written and read past the caches of the compute
+// dies (agent scope), and one has arrived in memory before its workgroup does at
+// the tickets: s_waitcnt is what the workgroup fence is here. (A release at agent
+// scope would write back what the dies' caches hold of others' data too, once a
+// workgroup: 45 us for ResNet-50's gradient instead of 18.)
 __global__ __launch_bounds__(kBlock) void norm_kernel(const Spans spans,
-                                                      double* partials) {
+                                                      double* partials,
+                                                      unsigned* tickets,
+                                                      float* out) {
   double sum = 0;
   int span = 0;
   for (int c = blockIdx.x; c < spans.start[spans.count]; c += gridDim.x) {
@@ -562,7 +574,26 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(const Spans spans,
     }
   }
   sum = block_sum(sum);
-  if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+  if (tickets == nullptr) {
+    if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+    return;
+  }
+  __shared__ bool finish;
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(partials + blockIdx.x, sum, __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    finish = last(tickets, arrive(tickets));
+  }
+  __syncthreads();
+  if (!finish) return;
+  sum = 0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kBlock)
+    sum += __hip_atomic_load(partials + i, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) *out = (float)sqrt(sum);
 }
 
 __global__ __launch_bounds__(kBlock) void norm_finish_kernel(
@@ -603,8 +634,10 @@ int norm_blocks(const Spans& spans) {
   return chunks < kNormBlocks ? chunks : kNormBlocks;
 }
 
-void norm_partials(const Spans& spans, double* partials, hipStream_t stream) {
-  norm_kernel<<<norm_blocks(spans), kBlock, 0, stream>>>(spans, partials);
+void norm_partials(const Spans& spans, double* partials, unsigned* tickets,
+                   float* out, hipStream_t stream) {
+  norm_kernel<<<norm_blocks(spans), kBlock, 0, stream>>>(spans, partials,
+                                                         tickets, out);
 }
 
 void norm_finish(const double* partials, int count, float* out,

@@ -4,6 +4,7 @@
 // device, nothing waits for the device, and everything can be captured into a
 // graph.
 
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -13,7 +14,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
-#include <cmath>
+#include <map>
 #include <memory>
 #include <optional>
 #include <vector>
@@ -69,6 +70,24 @@ uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
+// The tensors of a Python list or tuple (the caller's, which holds them), null
+// for None.
+std::vector<const Tensor*> tensors_of(pybind11::handle given, bool none) {
+  PyObject* const sequence = given.ptr();
+  TORCH_CHECK(PyList_Check(sequence) || PyTuple_Check(sequence),
+              "expected a list or tuple of tensors");
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(sequence);
+  PyObject** const items = PySequence_Fast_ITEMS(sequence);
+  std::vector<const Tensor*> out((size_t)count, nullptr);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    if (none && items[i] == Py_None) continue;
+    TORCH_CHECK(THPVariable_Check(items[i]), "expected a tensor at place ", i,
+                " of the sequence");
+    out[(size_t)i] = &THPVariable_Unpack(items[i]);
+  }
+  return out;
+}
+
 bool capturing() {
   return c10::hip::currentStreamCaptureStatusMayInitCtx() !=
          c10::hip::CaptureStatus::None;
@@ -107,10 +126,11 @@ class Plan {
     lay_out();
   }
 
-  void step(const std::vector<std::optional<Tensor>>& grads, double lr,
+  void step(pybind11::handle given, double lr,
             double beta1, double beta2, double eps, double weight_decay,
             const std::optional<Tensor>& norm, double max_norm) {
     const size_t count = params_.size();
+    const auto grads = tensors_of(given, /*none=*/true);
     TORCH_CHECK(grads.size() == count, "adamw: ", count, " parameters, but ",
                 grads.size(), " gradients");
     const c10::Device device = params_[0].device();
@@ -126,10 +146,10 @@ class Plan {
       hyper.norm = norm->data_ptr<float>();
     }
     // Everything is checked before anything is launched.
-    std::vector<Tensor> held(count);
     std::vector<int> types(count, 0);
+    bool moved = false;
     for (size_t i = 0; i < count; ++i) {
-      if (!grads[i]) continue;
+      if (grads[i] == nullptr) continue;
       const Tensor& g = *grads[i];
       const Tensor& p = params_[i];
       TORCH_CHECK(g.layout() == torch::kStrided,
@@ -144,14 +164,21 @@ class Plan {
                   ", its parameter ", p.scalar_type(),
                   " (the same type, or fp32 parameters)");
       check_apart(g, "adamw: gradient");
-      held[i] = g.resolve_neg();
+      moved = moved || g.is_neg() || !same_layout(g, p);
     }
+    // Gradients in another order than their parameters, laid out like them.
+    std::vector<Tensor> copies(moved ? count : 0);
+    std::vector<const void*> at(count, nullptr);
     for (size_t i = 0; i < count; ++i) {
-      if (!held[i].defined() || same_layout(held[i], params_[i])) continue;
-      auto moved = torch::empty_strided(params_[i].sizes(),
-                                        params_[i].strides(),
-                                        held[i].options());
-      held[i] = moved.copy_(held[i]);
+      if (grads[i] == nullptr) continue;
+      const Tensor& g = *grads[i];
+      at[i] = g.data_ptr();
+      if (g.is_neg() || !same_layout(g, params_[i])) {
+        copies[i] = torch::empty_strided(params_[i].sizes(),
+                                         params_[i].strides(), g.options());
+        copies[i].copy_(g);
+        at[i] = copies[i].data_ptr();
+      }
     }
 
     const auto current = c10::hip::getCurrentHIPStream();
@@ -176,11 +203,11 @@ class Plan {
       adamw::Grads g{};
       bool any = false;
       for (size_t i = first; i < last; ++i) {
-        if (!held[i].defined()) continue;
+        if (grads[i] == nullptr) continue;
         const size_t k = i - first;
         any = true;
         // A tensor of no elements has a gradient all the same: any address.
-        g.g[k] = held[i].numel() > 0 ? held[i].data_ptr() : (const void*)work;
+        g.g[k] = params_[i].numel() > 0 ? at[i] : (const void*)work;
         g.types[k / 16] |= (uint32_t)types[i] << (2 * (k % 16));
       }
       if (!any) continue;
@@ -193,7 +220,7 @@ class Plan {
     }
     // What autograd has saved of the parameters is out of date.
     for (size_t i = 0; i < count; ++i)
-      if (held[i].defined() && !params_[i].is_inference())
+      if (grads[i] != nullptr && !params_[i].is_inference())
         params_[i].unsafeGetTensorImpl()->bump_version();
   }
 
@@ -358,28 +385,45 @@ class Plan {
   bool captured_ = false;
 };
 
-Tensor grad_norm(const std::vector<Tensor>& tensors) {
+// Counters of the norm's arrivals for what a stream runs one after the other.
+// (A captured graph may run beside its stream's later work: it has none, and
+// finishes the sum in a launch of its own.) Never destroyed.
+unsigned* stream_tickets(const c10::hip::HIPStream& stream,
+                         const c10::Device& device) {
+  static auto* all = new std::map<std::pair<int, hipStream_t>, Tensor>();
+  Tensor& t = (*all)[{(int)device.index(), stream.stream()}];
+  if (!t.defined())
+    t = torch::zeros({adamw::kTicketInts},
+                     torch::TensorOptions().device(device).dtype(
+                         torch::kInt32));
+  return reinterpret_cast<unsigned*>(t.data_ptr());
+}
+
+Tensor grad_norm(pybind11::handle given_list) {
+  const auto tensors = tensors_of(given_list, /*none=*/false);
   TORCH_CHECK(!tensors.empty(), "grad_norm: expected a tensor");
-  const c10::Device device = tensors[0].device();
-  TORCH_CHECK(tensors[0].is_cuda(), "grad_norm: expected GPU tensors");
+  const c10::Device device = tensors[0]->device();
+  TORCH_CHECK(tensors[0]->is_cuda(), "grad_norm: expected GPU tensors");
   c10::DeviceGuard guard(device);
-  const auto stream = c10::hip::getCurrentHIPStream().stream();
+  const auto current = c10::hip::getCurrentHIPStream();
+  const auto stream = current.stream();
 
   std::vector<std::unique_ptr<adamw::Spans>> launches;
   std::vector<Tensor> held;
+  held.reserve(tensors.size());
   const char* end = nullptr;  // of the last span
-  for (const Tensor& given : tensors) {
+  for (const Tensor* each : tensors) {
+    const Tensor& given = *each;
     TORCH_CHECK(given.layout() == torch::kStrided && given.device() == device,
                 "grad_norm: expected dense tensors on one device");
     const int type = dtype_of(given, "grad_norm");
     int64_t n = given.numel();
     if (n == 0) continue;
     // The order of the elements does not matter, only that there are no gaps.
-    Tensor t = given;
-    if (!t.is_non_overlapping_and_dense()) {
-      t = t.contiguous();
-      held.push_back(t);
-    }
+    if (!given.is_non_overlapping_and_dense())
+      held.push_back(given.contiguous());
+    const Tensor& t =
+        given.is_non_overlapping_and_dense() ? given : held.back();
     const char* ptr = (const char*)t.data_ptr();
     if (!launches.empty()) {
       auto& s = *launches.back();
@@ -424,14 +468,18 @@ Tensor grad_norm(const std::vector<Tensor>& tensors) {
   auto partials =
       torch::empty({std::max(count, 1)}, options.dtype(torch::kFloat64));
   double* at = partials.data_ptr<double>();
+  float* const result = out.data_ptr<float>();
+  const bool one = launches.size() == 1 && !capturing();
   for (auto& s : launches) {
-    adamw::norm_partials(*s, at, stream);
+    adamw::norm_partials(*s, at, one ? stream_tickets(current, device) : nullptr,
+                         result, stream);
     C10_HIP_CHECK(hipGetLastError());
     at += adamw::norm_blocks(*s);
   }
-  adamw::norm_finish(partials.data_ptr<double>(), count, out.data_ptr<float>(),
-                     stream);
-  C10_HIP_CHECK(hipGetLastError());
+  if (!one) {
+    adamw::norm_finish(partials.data_ptr<double>(), count, result, stream);
+    C10_HIP_CHECK(hipGetLastError());
+  }
   return out;
 }
 
