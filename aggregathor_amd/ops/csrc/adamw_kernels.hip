@@ -41,7 +41,6 @@ namespace adamw {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kQuads = kChunk / (4 * kBlock);  // quads of a thread
 
 // Four elements of T. Tensors start anywhere (a gradient is a view into the
 // flat gradient), so a quad is only aligned like its element: gfx950 loads and
@@ -360,7 +359,7 @@ __device__ __forceinline__ bool last(unsigned* tickets, unsigned arrived) {
   return atomicInc(tickets, lines - 1) == lines - 1;
 }
 
-template <int Bits, typename P, typename G, bool Full>
+template <int Bits, int Quads, typename P, typename G, bool Full>
 __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
                                              const int* steps,
                                              unsigned* tickets,
@@ -377,12 +376,12 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
   const int n = w.left;
 
   // All loads first: they are on their way while the step is counted.
-  typename P::Quad pq[kQuads];
-  typename G::Quad gq[kQuads];
-  f32x4 mq[kQuads], vq[kQuads];
-  uint32_t mw[kQuads], rw[kQuads], ms[kQuads], rs[kQuads];
+  typename P::Quad pq[Quads];
+  typename G::Quad gq[Quads];
+  f32x4 mq[Quads], vq[Quads];
+  uint32_t mw[Quads], rw[Quads], ms[Quads], rs[Quads];
 #pragma unroll
-  for (int q = 0; q < kQuads; ++q) {
+  for (int q = 0; q < Quads; ++q) {
     const int i = 4 * (q * kBlock + (int)threadIdx.x);
     if constexpr (Bits == 32) {
       mq[q] = load4<Full, F32>(m32, i, n);
@@ -404,7 +403,7 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
   const Common k = common(s, w.key, (uint32_t)step);
 
 #pragma unroll
-  for (int q = 0; q < kQuads; ++q) {
+  for (int q = 0; q < Quads; ++q) {
     const int i = 4 * (q * kBlock + (int)threadIdx.x);
     float p[4], g[4], m[4], v[4], denominator[4];
     widen<P>(pq[q], p);
@@ -446,19 +445,19 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
   }
 }
 
-template <int Bits, typename P, typename G>
+template <int Bits, int Quads, typename P, typename G>
 __device__ __forceinline__ void update_tensor(const Work& w, const void* grad,
                                               const int* steps,
                                               unsigned* tickets,
                                               unsigned& arrived,
                                               const Scalars& s) {
-  if (w.left == kChunk)
-    update_chunk<Bits, P, G, true>(w, grad, steps, tickets, arrived, s);
+  if (w.left == Quads * 4 * kBlock)
+    update_chunk<Bits, Quads, P, G, true>(w, grad, steps, tickets, arrived, s);
   else
-    update_chunk<Bits, P, G, false>(w, grad, steps, tickets, arrived, s);
+    update_chunk<Bits, Quads, P, G, false>(w, grad, steps, tickets, arrived, s);
 }
 
-template <int Bits>
+template <int Bits, int Quads>
 __global__ __launch_bounds__(kBlock) void update_kernel(
     const Work* __restrict__ work, long nwork, int first, int count, int* steps,
     unsigned* tickets, const Grads grads, const Scalars s) {
@@ -476,19 +475,19 @@ __global__ __launch_bounds__(kBlock) void update_kernel(
     const uint32_t type = (grads.types[at / 16] >> (2 * (at % 16))) & 3;
     switch (w.type * 4 + type) {
       case kF32 * 4 + kF32:
-        update_tensor<Bits, F32, F32>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F32, F32>(w, grad, steps, tickets, arrived, s);
         break;
       case kF32 * 4 + kBF16:
-        update_tensor<Bits, F32, BF16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F32, BF16>(w, grad, steps, tickets, arrived, s);
         break;
       case kF32 * 4 + kF16:
-        update_tensor<Bits, F32, F16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F32, F16>(w, grad, steps, tickets, arrived, s);
         break;
       case kBF16 * 4 + kBF16:
-        update_tensor<Bits, BF16, BF16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, BF16, BF16>(w, grad, steps, tickets, arrived, s);
         break;
       case kF16 * 4 + kF16:
-        update_tensor<Bits, F16, F16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F16, F16>(w, grad, steps, tickets, arrived, s);
         break;
     }
   }
@@ -608,9 +607,9 @@ __global__ __launch_bounds__(kBlock) void norm_finish_kernel(
 
 bool supported(int p, int g) { return p == g || p == kF32; }
 
-void update(int bits, const Work* work, long nwork, int first, int count,
-            int* steps, unsigned* tickets, const Grads& grads, const Hyper& h,
-            hipStream_t stream) {
+void update(int bits, long chunk, const Work* work, long nwork, int first,
+            int count, int* steps, unsigned* tickets, const Grads& grads,
+            const Hyper& h, hipStream_t stream) {
   const Scalars s = {h.beta1,
                      h.beta2,
                      (float)h.lr,
@@ -621,12 +620,12 @@ void update(int bits, const Work* work, long nwork, int first, int count,
                      (float)h.max_norm,
                      h.norm};
   const dim3 grid((unsigned)(nwork > 0 ? nwork : 1));
-  if (bits == 8)
-    update_kernel<8><<<grid, kBlock, 0, stream>>>(
-        work, nwork, first, count, steps, tickets, grads, s);
-  else
-    update_kernel<32><<<grid, kBlock, 0, stream>>>(
-        work, nwork, first, count, steps, tickets, grads, s);
+  auto* const kernel = bits == 32             ? update_kernel<32, 1>
+                       : chunk == kChunkSmall ? update_kernel<8, 1>
+                                              : update_kernel<8, 2>;
+  static_assert(kChunkSmall == 4 * kBlock && kChunkLarge == 8 * kBlock);
+  kernel<<<grid, kBlock, 0, stream>>>(work, nwork, first, count, steps, tickets,
+                                      grads, s);
 }
 
 int norm_blocks(const Spans& spans) {

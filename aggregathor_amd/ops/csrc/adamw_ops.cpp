@@ -212,7 +212,7 @@ class Plan {
       }
       if (!any) continue;
       const int64_t begin = work_start_[first];
-      adamw::update(bits_, work + begin, work_start_[last] - begin, (int)first,
+      adamw::update(bits_, chunk_, work + begin, work_start_[last] - begin, (int)first,
                     (int)(last - first), steps,
                     tickets + first / adamw::kMaxTensors * adamw::kTicketInts,
                     g, hyper, stream);
@@ -278,6 +278,9 @@ class Plan {
         bits_ == 8 ? torch::kFloat8_e4m3fn : torch::kFloat32;
     std::vector<adamw::Work> table(count), work;
     std::vector<int64_t> work_start(count + 1, 0);
+    int64_t total = 0;
+    for (const Tensor& p : params_) total += p.numel();
+    const int64_t chunk = adamw::chunk_of(bits_, total);
     std::vector<Range> written{range_of(steps_)};
     for (size_t i = 0; i < count; ++i) {
       const Tensor& p = params_[i];
@@ -316,7 +319,7 @@ class Plan {
         t.ms = reinterpret_cast<uint8_t*>(ms_[i].data_ptr());
         t.rs = reinterpret_cast<uint8_t*>(rs_[i].data_ptr());
       }
-      for (int64_t start = 0; start < n; start += adamw::kChunk) {
+      for (int64_t start = 0; start < n; start += chunk) {
         adamw::Work w = t;
         const int64_t state = start * (bits_ / 8);
         w.p = (char*)t.p + start * p.element_size();
@@ -327,7 +330,7 @@ class Plan {
           w.rs = t.rs + start / adamw::kGroup;
         }
         w.start = start;
-        w.left = (int)std::min<int64_t>(n - start, adamw::kChunk);
+        w.left = (int)std::min(n - start, chunk);
         work.push_back(w);
       }
       TORCH_CHECK(work.size() <= INT32_MAX, "adamw: too many elements");
@@ -356,6 +359,7 @@ class Plan {
     for (const Tensor& p : params_) numel_.push_back(p.numel());
     table_ = std::move(table);
     work_start_ = std::move(work_start);
+    chunk_ = chunk;
     written_ = std::move(written);
     captured_ = false;
   }
@@ -377,6 +381,7 @@ class Plan {
   uint32_t seed_;
   std::vector<adamw::Work> table_;  // each tensor's first
   std::vector<int64_t> work_start_;  // before each tensor's, in device_work_
+  int64_t chunk_ = 0;
   std::vector<int64_t> numel_;
   std::vector<Range> written_;
   Tensor device_work_, tickets_;

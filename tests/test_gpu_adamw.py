@@ -19,6 +19,8 @@ pytestmark = pytest.mark.gpu
 
 # Around a quad, a group, a workgroup's part, and several of these.
 SIZES = [1, 3, 4, 5, 31, 32, 33, 127, 1025, 4095, 4096, 4097, 0, 12289, 70001]
+# Past the size from which 8-bit states take larger parts, in all.
+LARGE = [2047, 2048, 1, 2049, 33, 2200001]
 HYPER = dict(lr=1e-2, beta1=0.9, beta2=0.99, eps=1e-6, weight_decay=0.1)
 TYPES = [(torch.float32, torch.float32), (torch.float32, torch.bfloat16),
          (torch.float32, torch.float16), (torch.bfloat16, torch.bfloat16),
@@ -166,10 +168,11 @@ def test_step32(p_dtype, g_dtype, max_norm):
 
 @pytest.mark.parametrize("max_norm", [None, 0.5])
 @pytest.mark.parametrize("p_dtype,g_dtype", TYPES)
-def test_step8(p_dtype, g_dtype, max_norm):
-    params, grads = _tensors(SIZES, p_dtype), _tensors(SIZES, g_dtype, 5, 0.3)
-    state = _state8(SIZES)
-    counts = [(37 * i) % 1000 for i in range(len(SIZES))]
+@pytest.mark.parametrize("sizes", [SIZES, LARGE])
+def test_step8(sizes, p_dtype, g_dtype, max_norm):
+    params, grads = _tensors(sizes, p_dtype), _tensors(sizes, g_dtype, 5, 0.3)
+    state = _state8(sizes)
+    counts = [(37 * i) % 1000 for i in range(len(sizes))]
     values = [(R.values8(a, b), R.values8(c, d).square())
               for a, b, c, d in zip(*state)]
     s = 1. if max_norm is None else oracle.clip_factor(grads, max_norm)[1]
@@ -188,7 +191,7 @@ def test_step8(p_dtype, g_dtype, max_norm):
         norm=None if max_norm is None else ops.grad_norm(grads))
     assert steps.tolist() == [t + 1 for t in counts]
     for i, (x, bounds) in enumerate(want):
-        what = f"of {SIZES[i]}"
+        what = f"of {sizes[i]}"
         oracle.check(p[i], x[0], oracle.rounded(bounds[0], x[0], p_dtype),
                      "p " + what)
         _check_states([c[i] for c in own], [c[i] for c in state], what)
