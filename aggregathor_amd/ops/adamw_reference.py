@@ -60,6 +60,11 @@ def state8(param):
 
 
 def values8(codes, scales):
+    if codes.dtype != torch.float8_e4m3fn or not _dense(codes) or \
+            scales.dtype != torch.float8_e8m0fnu or \
+            scales.shape != (_groups(codes.numel()),):
+        raise RuntimeError("adamw: expected dense e4m3 codes and an e8m0 scale "
+                           f"for every {GROUP} of them")
     out = torch.empty_like(codes, dtype=torch.float32)
     n = codes.numel()
     scaled = _grouped(_flat(codes).float()) * scales.float()[:, None]

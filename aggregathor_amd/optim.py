@@ -75,7 +75,11 @@ class AdamW(torch.optim.Optimizer):
     def _lay_out(self):
         """Make the states that are missing, and a plan for each group (and
         each device of its parameters)."""
-        self._plans, self._first_steps = [], []
+        if torch.cuda.is_available() and \
+                torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("adamw: run a step before the capture, so that "
+                               "the states and plans are there")
+        plans, first_steps = [], []
         for index, group in enumerate(self.param_groups):
             self._check_bits(group)
             bits = group["state_bits"]
@@ -104,8 +108,9 @@ class AdamW(torch.optim.Optimizer):
                                            seed=self.rounding_seed + index)
                 else:
                     plan = ops.adamw_plan(params, *columns, steps)
-                self._plans.append((group, params, plan))
-                self._first_steps.append(self.state[params[0]]["step"])
+                plans.append((group, params, plan))
+                first_steps.append(self.state[params[0]]["step"])
+        self._plans, self._first_steps = plans, first_steps
 
     def _state_kept(self):
         """Whether the plans still hold the state (a user may have cleared it;
@@ -170,19 +175,21 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("loaded state dict lacks " + ", ".join(
                 sorted(missing)) + f" of a state of {bits} bits")
         out = {"step": torch.as_tensor(state["step"]).to(torch.int32)}
+        names = _STATES[32] if bits == 32 else ("exp_avg", "exp_avg_root")
+        for name in names:
+            if state[name].shape != p.shape:
+                raise ValueError(f"loaded {name} has the shape "
+                                 f"{tuple(state[name].shape)}, its parameter "
+                                 f"{tuple(p.shape)}")
         if bits == 32:
-            for name in _STATES[32]:
+            for name in names:
                 out[name] = torch.empty_like(
                     p, dtype=torch.float32, requires_grad=False).copy_(
                         state[name])
             return out
-        for name in ("exp_avg", "exp_avg_root"):
+        for name in names:
             codes = state[name]
             scales = state[name + "_scale"]
-            if codes.shape != p.shape:
-                raise ValueError(f"loaded {name} has the shape "
-                                 f"{tuple(codes.shape)}, its parameter "
-                                 f"{tuple(p.shape)}")
             if codes.dtype != torch.float8_e4m3fn or \
                     scales.dtype != torch.float8_e8m0fnu:
                 raise ValueError(f"loaded {name} is no 8-bit state")

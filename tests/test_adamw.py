@@ -453,6 +453,47 @@ def test_optimizer_refuses():
         AdamW(list(model.parameters())[1:]).load_state_dict(opt.state_dict())
 
 
+def test_loading_does_not_stretch_states():
+    model = _model()
+    opt = AdamW(model.parameters())
+    _train(model, opt, 1)
+    state = opt.state_dict()
+    state["state"][0]["exp_avg"] = torch.zeros(1)
+    with pytest.raises(ValueError, match="shape"):
+        AdamW(model.parameters()).load_state_dict(state)
+
+
+def test_values_refuse():
+    codes, scales, *_ = ops.adamw8_state(torch.zeros(100))
+    assert torch.equal(ops.adamw8_values(codes, scales), torch.zeros(100))
+    for a, b in ((codes.float(), scales), (codes[::2], scales[:2]),
+                 (codes, scales[:3]), (codes, scales.float())):
+        with pytest.raises(RuntimeError):
+            ops.adamw8_values(a, b)
+
+
+def test_any_iterable_of_tensors():
+    args = _plan_args(bits=32)
+    plan = ops.adamw_plan(*args)
+    ops.adamw_step(plan, (g for g in [torch.ones(40)]), lr=0.1)
+    ops.adamw_step(plan, (torch.ones(40),), lr=0.1)
+    assert int(args[3]) == 2
+    assert float(ops.grad_norm(t for t in [torch.ones(9)])) == 3
+
+
+def test_schedulers_reach_the_step():
+    p = torch.nn.Parameter(torch.ones(()))
+    opt = AdamW([p], lr=1., weight_decay=0.)
+    schedule = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.)
+    p.grad = torch.ones(())
+    opt.step()
+    schedule.step()
+    before = p.detach().clone()
+    assert float(before) == pytest.approx(0., abs=1e-6)
+    opt.step()
+    assert torch.equal(p, before)
+
+
 def test_groups_with_their_own_settings():
     model = _model()
     params = list(model.parameters())

@@ -467,6 +467,70 @@ def test_other_streams_and_a_plan_that_ends(bits):
         assert torch.equal(a, b)
 
 
+def test_norms_on_streams_at_once():
+    # Each with its own counters: many in flight on several streams, and beside
+    # them a graph's.
+    xs = [torch.randn(3_000_000 + 1000 * k, device="cuda") for k in range(4)]
+    want = [ops.grad_norm(x) for x in xs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = ops.grad_norm(xs[0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[] for _ in xs]
+    for _ in range(20):
+        for x, stream, out in zip(xs, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(ops.grad_norm(x))
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(inside, want[0])
+    for w, out in zip(want, got):
+        assert all(torch.equal(w, x) for x in out)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_elements_and_no_dimensions(bits):
+    make = ops.adamw8_plan if bits == 8 else ops.adamw_plan
+    empty = [torch.zeros(0, device="cuda"), torch.zeros(3, 0, device="cuda")]
+
+    def state(p):
+        return ops.adamw8_state(p) if bits == 8 else [torch.zeros_like(p)
+                                                      for _ in range(2)]
+    for params in (empty, [torch.ones((), device="cuda")] + empty):
+        steps = torch.zeros(len(params), dtype=torch.int32, device="cuda")
+        plan = make(params, *[list(c) for c in zip(*map(state, params))],
+                    steps)
+        for k in range(3):
+            ops.adamw_step(plan, [None] * len(params), lr=0.5)
+            ops.adamw_step(plan, [torch.ones_like(p) for p in params], lr=0.5,
+                           weight_decay=0.)
+            assert steps.tolist() == [k + 1] * len(params)
+    # Three steps of 0.5 from 1. A code is off by an eighth at most: with 8 bits m
+    # is off by 0.9 * 0.1 / 0.19 / 8 = 0.06 in the second step and by (0.06 +
+    # 0.125) 0.9 * 0.19 / 0.271 = 0.12 in the third, r by 0.07 and 0.14 (half of
+    # v's 0.5 * 0.266 and 0.667 * 0.43), so the steps by 0.14 and 0.3 of 0.5.
+    assert float(params[0]) == pytest.approx(
+        -0.5, abs=1e-5 if bits == 32 else 0.22)
+
+
+def test_a_capture_before_the_first_step_is_refused():
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = AdamW([p], lr=0.5, weight_decay=0.)
+    p.grad = torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    assert int(opt.state[p]["step"]) == 2
+    torch.testing.assert_close(p.detach(), torch.zeros(8, device="cuda"),
+                               rtol=0, atol=1e-5)
+
+
 def test_parameters_that_moved():
     plan, params, state, steps, grads = _small_plan(32)
     want = _small_plan(32)
