@@ -390,18 +390,26 @@ class Plan {
   bool captured_ = false;
 };
 
-// Counters of the norm's arrivals for what a stream runs one after the other.
-// (A captured graph may run beside its stream's later work: it has none, and
-// finishes the sum in a launch of its own.) Never destroyed.
-unsigned* stream_tickets(const c10::hip::HIPStream& stream,
-                         const c10::Device& device) {
-  static auto* all = new std::map<std::pair<int, hipStream_t>, Tensor>();
-  Tensor& t = (*all)[{(int)device.index(), stream.stream()}];
-  if (!t.defined())
-    t = torch::zeros({adamw::kTicketInts},
-                     torch::TensorOptions().device(device).dtype(
-                         torch::kInt32));
-  return reinterpret_cast<unsigned*>(t.data_ptr());
+// Counters of the norm's arrivals, and room for its partial sums, for what a
+// stream runs one after the other. (A captured graph may run beside its stream's
+// later work: it has sums of its own, and adds them up in a launch of its own.)
+// Never destroyed.
+struct NormSpace {
+  Tensor tickets, partials;
+};
+
+const NormSpace& norm_space(const c10::hip::HIPStream& stream,
+                            const c10::Device& device) {
+  static auto* all = new std::map<std::pair<int, hipStream_t>, NormSpace>();
+  NormSpace& space = (*all)[{(int)device.index(), stream.stream()}];
+  if (!space.partials.defined()) {
+    const auto options = torch::TensorOptions().device(device);
+    space.tickets =
+        torch::zeros({adamw::kTicketInts}, options.dtype(torch::kInt32));
+    space.partials =
+        torch::empty({adamw::kNormBlocks}, options.dtype(torch::kFloat64));
+  }
+  return space;
 }
 
 Tensor grad_norm(pybind11::handle given_list) {
@@ -468,23 +476,27 @@ Tensor grad_norm(pybind11::handle given_list) {
   }
   auto options = torch::TensorOptions().device(device);
   auto out = torch::empty({}, options.dtype(torch::kFloat32));
+  float* const result = out.data_ptr<float>();
+  if (launches.size() == 1 && !capturing()) {
+    const NormSpace& space = norm_space(current, device);
+    adamw::norm_partials(*launches[0], space.partials.data_ptr<double>(),
+                         reinterpret_cast<unsigned*>(space.tickets.data_ptr()),
+                         result, stream);
+    C10_HIP_CHECK(hipGetLastError());
+    return out;
+  }
   int count = 0;
   for (auto& s : launches) count += adamw::norm_blocks(*s);
   auto partials =
       torch::empty({std::max(count, 1)}, options.dtype(torch::kFloat64));
   double* at = partials.data_ptr<double>();
-  float* const result = out.data_ptr<float>();
-  const bool one = launches.size() == 1 && !capturing();
   for (auto& s : launches) {
-    adamw::norm_partials(*s, at, one ? stream_tickets(current, device) : nullptr,
-                         result, stream);
+    adamw::norm_partials(*s, at, nullptr, result, stream);
     C10_HIP_CHECK(hipGetLastError());
     at += adamw::norm_blocks(*s);
   }
-  if (!one) {
-    adamw::norm_finish(partials.data_ptr<double>(), count, result, stream);
-    C10_HIP_CHECK(hipGetLastError());
-  }
+  adamw::norm_finish(partials.data_ptr<double>(), count, result, stream);
+  C10_HIP_CHECK(hipGetLastError());
   return out;
 }
 
