@@ -503,6 +503,9 @@ __global__ __launch_bounds__(kBlock) void update_kernel(
 // fp32 overflows or vanishes, and the vector units have the rate for it at
 // four bytes an element. Which workgroup adds which elements is fixed by the
 // spans alone, so the result is the same every time.
+// Loads are not nontemporal here: a step reads the same gradients next. (Clipped
+// VGG-16 697 us instead of 722, ResNet-50 with 8-bit states 88 instead of 91; the
+// norms by themselves 46.7 and 19.9 us instead of 43.6 and 18.9.)
 
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const void* ptr, int chunk,
@@ -516,7 +519,9 @@ __device__ __forceinline__ double chunk_squares(const void* ptr, int chunk,
 #pragma unroll
     for (int q = 0; q < kElems / (4 * kBlock); ++q) {
       float x[4];
-      widen<T>(load4<true, T>(base, 4 * (q * kBlock + (int)threadIdx.x), 0), x);
+      widen<T>(*(Global<const typename T::Quad>)(
+                   base + 4 * (q * kBlock + (int)threadIdx.x)),
+               x);
 #pragma unroll
       for (int c = 0; c < 4; ++c) sum[c] = fma((double)x[c], (double)x[c], sum[c]);
     }
