@@ -13,12 +13,13 @@ enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
 // Elements that share one scale in an 8-bit state.
 constexpr int kGroup = 32;
-// Elements that one workgroup updates: few, so that its registers leave room for
-// eight waves a SIMD and small tensors spread out. With 8-bit states, whose vector
-// work is what the memory barely hides, two quads a thread share what a workgroup
-// computes once, where there is enough to fill the card all the same (four
-// workgroups a CU). Measured, 1024 / 2048 a workgroup: 8 bits 1.8M elements 8.3 /
-// 8.5 us, 3.5M 15.9 / 14.1, 47M 141 / 128; 32 bits 80k 4.0 / 4.4, 26M 116 / 118.
+// Elements that one workgroup updates: few, so that its registers leave room
+// for eight waves a SIMD and small tensors spread out. With 8-bit states, whose
+// vector work is what the memory barely hides, two quads a thread share what a
+// workgroup computes once, where there is enough to fill the card all the same
+// (four workgroups a CU). Measured, 1024 / 2048 a workgroup: 8 bits 1.8M
+// elements 8.3 / 8.5 us, 3.5M 15.9 / 14.1, 47M 141 / 128; 32 bits 80k 4.0 / 4.4,
+// 26M 116 / 118.
 constexpr long kChunkSmall = 1024, kChunkLarge = 2048;
 
 inline long chunk_of(int bits, long elements) {
@@ -37,9 +38,13 @@ constexpr int kMaxSpans = 160;
 constexpr int kNormBlocks = 768;
 constexpr int kNormChunkBytes = 16384;
 
+// Workgroups of one launch: the threads of a grid's dimension are counted in 32
+// bits.
+constexpr long kMaxWork = (1l << 32) / 256 - 1;
+
 // What one workgroup updates: `left` elements of a tensor from the element
-// `start` on (a multiple of the chunk), where the pointers point. All that it needs
-// is in one place, so that its first loads of data wait for one load only.
+// `start` on (a multiple of the chunk), where the pointers point. All that it
+// needs is in one place, so that its first loads of data wait for one load only.
 // 32-bit states: m and r point to floats (r to the mean square itself), ms and
 // rs are null. 8-bit states: m and r point to e4m3 codes (r to those of the mean
 // square's root), ms and rs to their groups' biased exponents.
@@ -81,8 +86,8 @@ constexpr int kTicketInts = 32 * (kTicketLines + 1);
 // One AdamW step of the tensors [first, first + count): steps[i] += 1 for those
 // that have a gradient. work[0..nwork) is all that there is to do for them, in
 // parts of at most `chunk`, and grads.g[i] belongs to tensor first + i.
-void update(int bits, long chunk, const Work* work, long nwork, int first, int count,
-            int* steps, unsigned* tickets, const Grads& grads,
+void update(int bits, long chunk, const Work* work, long nwork, int first,
+            int count, int* steps, unsigned* tickets, const Grads& grads,
             const Hyper& hyper, hipStream_t stream);
 
 // Spans of elements that lie back to back in memory: start[i] is the first

@@ -342,7 +342,7 @@ __device__ __forceinline__ Common common(const Scalars& s, uint32_t key,
 // 4 us a step.) One address takes an arrival in 12 ns, so they arrive at 32, and
 // the last of each of these at one. Counters wrap by themselves to the zero that
 // the next launch needs.
-__device__ __forceinline__ unsigned on_line() {  // workgroups of this one's line
+__device__ __forceinline__ unsigned on_line() {  // workgroups that share one
   return (gridDim.x - blockIdx.x % kTicketLines + kTicketLines - 1) /
          kTicketLines;
 }
@@ -454,7 +454,8 @@ __device__ __forceinline__ void update_tensor(const Work& w, const void* grad,
   if (w.left == Quads * 4 * kBlock)
     update_chunk<Bits, Quads, P, G, true>(w, grad, steps, tickets, arrived, s);
   else
-    update_chunk<Bits, Quads, P, G, false>(w, grad, steps, tickets, arrived, s);
+    update_chunk<Bits, Quads, P, G, false>(w, grad, steps, tickets, arrived,
+                                           s);
 }
 
 template <int Bits, int Quads>
@@ -475,19 +476,24 @@ __global__ __launch_bounds__(kBlock) void update_kernel(
     const uint32_t type = (grads.types[at / 16] >> (2 * (at % 16))) & 3;
     switch (w.type * 4 + type) {
       case kF32 * 4 + kF32:
-        update_tensor<Bits, Quads, F32, F32>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F32, F32>(w, grad, steps, tickets, arrived,
+                                           s);
         break;
       case kF32 * 4 + kBF16:
-        update_tensor<Bits, Quads, F32, BF16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F32, BF16>(w, grad, steps, tickets, arrived,
+                                           s);
         break;
       case kF32 * 4 + kF16:
-        update_tensor<Bits, Quads, F32, F16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F32, F16>(w, grad, steps, tickets, arrived,
+                                           s);
         break;
       case kBF16 * 4 + kBF16:
-        update_tensor<Bits, Quads, BF16, BF16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, BF16, BF16>(w, grad, steps, tickets, arrived,
+                                           s);
         break;
       case kF16 * 4 + kF16:
-        update_tensor<Bits, Quads, F16, F16>(w, grad, steps, tickets, arrived, s);
+        update_tensor<Bits, Quads, F16, F16>(w, grad, steps, tickets, arrived,
+                                           s);
         break;
     }
   }

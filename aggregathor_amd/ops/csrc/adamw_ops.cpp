@@ -95,7 +95,7 @@ bool capturing() {
 
 // Tables that a captured graph reads stay for the process's life: a replay
 // after the plan is gone would take addresses from memory that is something
-// else by then. A few KiB each. Never destroyed.
+// else by then. 64 bytes for 1024 elements or 2048. Never destroyed.
 std::vector<Tensor>& captured_tables() {
   static auto* kept = new std::vector<Tensor>();
   return *kept;
@@ -122,13 +122,14 @@ class Plan {
         rs_(std::move(rs)),
         steps_(std::move(steps)),
         seed_((uint32_t)seed) {
+    TORCH_CHECK(bits_ == 8 || bits_ == 32, "adamw: states have 8 or 32 bits");
     TORCH_CHECK(!params_.empty(), "adamw: a plan needs a parameter");
     lay_out();
   }
 
-  void step(pybind11::handle given, double lr,
-            double beta1, double beta2, double eps, double weight_decay,
-            const std::optional<Tensor>& norm, double max_norm) {
+  void step(pybind11::handle given, double lr, double beta1, double beta2,
+            double eps, double weight_decay, const std::optional<Tensor>& norm,
+            double max_norm) {
     const size_t count = params_.size();
     const auto grads = tensors_of(given, /*none=*/true);
     TORCH_CHECK(grads.size() == count, "adamw: ", count, " parameters, but ",
@@ -212,8 +213,8 @@ class Plan {
       }
       if (!any) continue;
       const int64_t begin = work_start_[first];
-      adamw::update(bits_, chunk_, work + begin, work_start_[last] - begin, (int)first,
-                    (int)(last - first), steps,
+      adamw::update(bits_, chunk_, work + begin, work_start_[last] - begin,
+                    (int)first, (int)(last - first), steps,
                     tickets + first / adamw::kMaxTensors * adamw::kTicketInts,
                     g, hyper, stream);
       C10_HIP_CHECK(hipGetLastError());
@@ -266,7 +267,8 @@ class Plan {
     const size_t count = params_.size();
     const c10::Device device = params_[0].device();
     TORCH_CHECK(m_.size() == count && r_.size() == count &&
-                    (bits_ == 32 || (ms_.size() == count && rs_.size() == count)),
+                    (bits_ == 32 ||
+                     (ms_.size() == count && rs_.size() == count)),
                 "adamw: as many states as parameters are needed");
     TORCH_CHECK(steps_.device() == device && steps_.dim() == 1 &&
                     steps_.size(0) == (int64_t)count &&
@@ -333,8 +335,11 @@ class Plan {
         w.left = (int)std::min(n - start, chunk);
         work.push_back(w);
       }
-      TORCH_CHECK(work.size() <= INT32_MAX, "adamw: too many elements");
       work_start[i + 1] = (int64_t)work.size();
+      TORCH_CHECK(work_start[i + 1] -
+                          work_start[i - i % adamw::kMaxTensors] <=
+                      adamw::kMaxWork,
+                  "adamw: too many elements for one launch");
     }
     std::sort(written.begin(), written.end(),
               [](const Range& a, const Range& b) { return a.lo < b.lo; });

@@ -129,6 +129,8 @@ def test_grad_norm_extremes():
         got = float(ops.grad_norm(torch.full((n,), value, device="cuda")))
         assert got == pytest.approx(want, rel=1e-6, nan_ok=True)
     assert float(ops.grad_norm([torch.zeros(0, device="cuda")])) == 0
+    three = torch.full((9,), 1., device="cuda")
+    assert float(ops.grad_norm([three] * 4)) == 6
 
 
 def test_grad_norm_large():
