@@ -342,21 +342,24 @@ __device__ __forceinline__ Common common(const Scalars& s, uint32_t key,
 // 4 us a step.) One address takes an arrival in 12 ns, so they arrive at 32, and
 // the last of each of these at one. Counters wrap by themselves to the zero that
 // the next launch needs.
+// Up to 64 of them arrive at one at once: a second arrival would take longer
+// than they wait for each other.
+__device__ __forceinline__ unsigned lines() {
+  return gridDim.x <= 64 ? 1 : kTicketLines;
+}
+
 __device__ __forceinline__ unsigned on_line() {  // workgroups that share one
-  return (gridDim.x - blockIdx.x % kTicketLines + kTicketLines - 1) /
-         kTicketLines;
+  return (gridDim.x - blockIdx.x % lines() + lines() - 1) / lines();
 }
 
 __device__ __forceinline__ unsigned arrive(unsigned* tickets) {
-  return atomicInc(tickets + 32 * (1 + blockIdx.x % kTicketLines),
-                   on_line() - 1);
+  return atomicInc(tickets + 32 * (1 + blockIdx.x % lines()), on_line() - 1);
 }
 
 // Whether this workgroup, given what arrive() returned, was the last.
 __device__ __forceinline__ bool last(unsigned* tickets, unsigned arrived) {
   if (arrived != on_line() - 1) return false;
-  const unsigned lines = gridDim.x < kTicketLines ? gridDim.x : kTicketLines;
-  return atomicInc(tickets, lines - 1) == lines - 1;
+  return lines() == 1 || atomicInc(tickets, lines() - 1) == lines() - 1;
 }
 
 template <int Bits, int Quads, typename P, typename G, bool Full>
