@@ -2,8 +2,7 @@
 the CPU path, and what the HIP kernels are compared with.
 
 States are computed in the kernels' order, one rounding an operation, so that
-they come out the same bit by bit, but for codes of a root where the kernels'
-square root is off in its last bit and the rounding is next to a border.
+they come out the same bit by bit.
 """
 
 import torch
@@ -265,7 +264,8 @@ class Plan:
             v = _flat(values8(rs, self.rs[i])).square()
         m = m * beta1 + g * (1 - beta1)
         v = v * beta2 + g * g * (1 - beta2)
-        root = v.sqrt()
+        # Through 64 bits: the CPU's vector library is off in the last one.
+        root = v.double().sqrt().float()
         moved = (_flat(p).float() * (1 - lr * weight_decay)
                  - rate * (m / (root * unbias + eps)))
         # copy_ through the parameter, so that autograd sees the change.

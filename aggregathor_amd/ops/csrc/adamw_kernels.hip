@@ -22,13 +22,14 @@
 // its inputs, the same on every rank and in every replay.
 // The step itself uses the new m and v before they are rounded.
 //
-// m, v and the scales are plain IEEE fp32, one rounding an operation (no
-// contraction into fused multiply-adds), so they can be compared with another
-// implementation's bit by bit. The root and the quotient take the hardware's
-// square root and reciprocal, which are off by a unit in the last place at most
-// (seen over all normal numbers): the full sequences for the last half bit are
-// 25 instructions an element, and with 8-bit states the vector units were as
-// busy as the memory (114 instructions an element for 16 bytes).
+// m, v, scales and codes are those of plain IEEE fp32, one rounding an operation
+// (no contraction into fused multiply-adds), so that states can be compared with
+// another implementation's bit by bit. The quotient takes the hardware's
+// reciprocal, and with 32-bit states the root its square root, which are off by
+// a unit in the last place at most (seen over all normal numbers): with 8-bit
+// states the vector units are as busy as the memory, at 80 instructions an
+// element for 16 bytes (114 with the full sequences for quotient, root and
+// rounding took 411 us for VGG-16 where this takes 360).
 
 #include <hip/hip_runtime.h>
 
@@ -247,10 +248,14 @@ __device__ __forceinline__ Codes encode_states(const Common& k, long at,
   for (int c = 0; c < 4; ++c) {
     const uint32_t h = mix((uint32_t)(at + c) ^ key);
     zm[c] = copysignf(round_by_chance(fabsf(m[c]) * im, h & 0xFFFFu), m[c]);
-    // v / scale^2 first: the hardware's root takes denormals for zero. What is
-    // still one is 2^71 below the group's largest root, and raised to that.
-    const float y = __builtin_amdgcn_sqrtf(
-        fmaxf(ldexpf(v[c], 2 * (7 - half)), 0x1p-126f));
+    // v / scale^2, its root and the root's last bit, which is right for all that
+    // is above 2^-100 (tried for every such number). What is below 2^-126, whose
+    // root is 2^71 below the group's largest, is raised to that: the hardware
+    // takes denormals for zero.
+    const float x = fmaxf(ldexpf(v[c], 2 * (7 - half)), 0x1p-126f);
+    const float over = __builtin_amdgcn_rsqf(x), near = x * over;
+    const float y = __builtin_fmaf(__builtin_fmaf(-near, near, x), 0.5f * over,
+                                   near);
     denominator[c] = __builtin_fmaf(y, root_unit, k.eps);
     zr[c] = fmaxf(round_by_chance(y, h >> 16), v[c] > 0.f ? 0x1p-9f : 0.f);
     if (!Plain) {
