@@ -7,8 +7,8 @@ by side, and one that links them into one in-tree .so.)
 
 Direct hipcc invocations (no hipify, no CUDA compatibility machinery): the
 kernels are native HIP/CDNA4 and the glue uses the c10::hip API directly.
-The resulting ``_gar_hip.so`` is written next to this file so it ships with
-the repo snapshot to GPU boxes (it is .gitignore'd, not .gpurunignore'd).
+The resulting ``_gar_hip.so`` is written next to this file, so that a copy of the
+tree has it (git ignores it).
 
 Usage: ``python -m aggregathor_amd.ops.build`` (re-builds only when sources
 are newer than the .so; ``--force`` to rebuild).
