@@ -149,10 +149,15 @@ class AdamW(torch.optim.Optimizer):
         """Load what :meth:`state_dict` gave. (The base class would cast every
         state to its parameter's type.)"""
         groups = []
-        for group in state_dict["param_groups"]:
-            group = dict(group)
-            group.setdefault("state_bits", 32)
+        for given in state_dict["param_groups"]:
+            group = {**self.defaults, **given}
+            if state_dict["state"] and "state_bits" not in given:
+                group["state_bits"] = 32  # torch's own
             self._check_bits(group)
+            for other in ("amsgrad", "maximize"):
+                if group.get(other):
+                    raise ValueError(f"loaded state dict is of a step with "
+                                     f"{other}, which this optimizer has not")
             groups.append(group)
         saved = [i for group in groups for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]

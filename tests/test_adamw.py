@@ -437,6 +437,27 @@ def test_loads_torchs_state():
         torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-6)
 
 
+def test_loads_only_what_it_can_go_on_with():
+    model = _model()
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        other = torch.optim.AdamW(model.parameters(), **kw)
+        _train(model, other, 1)
+        with pytest.raises(ValueError):
+            AdamW(model.parameters()).load_state_dict(other.state_dict())
+    sgd = torch.optim.SGD(model.parameters(), lr=0.5, momentum=0.9)
+    _train(model, sgd, 1)
+    with pytest.raises(ValueError):
+        AdamW(model.parameters()).load_state_dict(sgd.state_dict())
+    # Without states there is nothing to go on with but the settings.
+    opt = AdamW(model.parameters(), eps=1e-6, state_bits=8)
+    opt.load_state_dict(torch.optim.SGD(model.parameters(),
+                                        lr=0.5).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
+    assert opt.param_groups[0]["eps"] == 1e-6
+    assert opt.param_groups[0]["state_bits"] == 8
+    _train(model, opt, 1)
+
+
 def test_optimizer_refuses():
     model = _model()
     with pytest.raises(tools.UserException):
