@@ -4,6 +4,10 @@
 import copy
 import io
 import math
+import os
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -560,3 +564,23 @@ def test_engine_steps_and_resumes(args):
     two.step()
     for p, q in zip(one.params, two.params):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_ranks_stay_alike(tmp_path, bits):
+    worker = pathlib.Path(__file__).parent / "adamw_dist_worker.py"
+    outs = [tmp_path / f"rank{rank}.pt" for rank in range(2)]
+    procs = [subprocess.Popen(
+        [sys.executable, str(worker), str(out), f"state-bits:{bits}"],
+        env={**os.environ, "RANK": str(rank), "WORLD_SIZE": "2",
+             "LOCAL_RANK": str(rank), "MASTER_ADDR": "127.0.0.1",
+             "MASTER_PORT": str(29700 + bits), "GLOO_SOCKET_IFNAME": "lo"},
+        stdout=subprocess.PIPE, stderr=subprocess.PIPE)
+        for rank, out in enumerate(outs)]
+    for p in procs:
+        _, err = p.communicate(timeout=300)
+        assert p.returncode == 0, err.decode()[-2000:]
+    one, two = (torch.load(out, weights_only=True) for out in outs)
+    for a, b in zip(one, two):
+        assert len(a) == len(b) == (4 if bits == 32 else 6)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
