@@ -246,6 +246,36 @@ def test_nan_infinity_zero_and_denormals(bits):
     torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-8, equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_are_not_finite(bits, dtype):
+    p = torch.tensor([math.nan, math.inf, -math.inf, 1., -0.], device="cuda",
+                     dtype=dtype)
+    opt = AdamW([p], lr=0.5, weight_decay=0.5, state_bits=bits)
+    p.grad = torch.zeros(5, device="cuda", dtype=dtype)
+    opt.step()
+    assert p[0].isnan()
+    assert p[1:].tolist() == [math.inf, -math.inf, 0.75, 0.]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_plain_form_on_the_gpu(bits, monkeypatch):
+    kernel = _small_plan(bits)
+    monkeypatch.setenv("AGGREGATHOR_FORCE_EAGER", "1")
+    plain = _small_plan(bits)
+    assert isinstance(plain[0], R.Plan)
+    for plan, params, state, steps, grads in (kernel, plain):
+        norm = ops.grad_norm(grads)
+        for _ in range(2):
+            ops.adamw_step(plan, grads, **HYPER, norm=norm, max_norm=0.5)
+    assert torch.equal(kernel[3], plain[3])
+    for a, b in zip(kernel[2], plain[2]):
+        assert all(_equal(x, y) for x, y in zip(a, b))
+    for a, b in zip(kernel[1], plain[1]):
+        torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-6)
+
+
 @pytest.mark.parametrize("norm", [0., math.inf, math.nan])
 def test_norms_that_are_none(norm):
     p = torch.ones(5, device="cuda")
