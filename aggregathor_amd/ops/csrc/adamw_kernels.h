@@ -34,7 +34,7 @@ constexpr int kMaxTensors = 448;
 // (three a CU), and the bytes that one of them reads at a time. Measured for
 // VGG-16's bf16 gradient: 512, 768, 1024, 2048 workgroups 52, 46.7, 47.7, 50.5
 // us; 8192, 16384, 32768 bytes 54, 47.7, 48.8 us.
-constexpr int kMaxSpans = 160;
+constexpr int kMaxSpans = 176;
 constexpr int kNormBlocks = 768;
 constexpr int kNormChunkBytes = 16384;
 
@@ -90,14 +90,13 @@ void update(int bits, long chunk, const Work* work, long nwork, int first,
             int count, int* steps, unsigned* tickets, const Grads& grads,
             const Hyper& hyper, hipStream_t stream);
 
-// Spans of elements that lie back to back in memory: start[i] is the first
-// chunk (of kNormChunkBytes) of span i within the launch, start[count] their
-// number.
+// Spans of elements that lie back to back in memory: n4t[i] is four times the
+// number of elements of span i, and its type; start[i] is its first chunk (of
+// kNormChunkBytes) within the launch, start[count] the number of chunks.
 struct Spans {
   const void* ptr[kMaxSpans];
-  long n[kMaxSpans];
+  long n4t[kMaxSpans];
   int start[kMaxSpans + 1];
-  int type[kMaxSpans];
   int count;
 };
 

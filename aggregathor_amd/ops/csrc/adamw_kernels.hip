@@ -579,15 +579,16 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(const Spans spans,
   for (int c = blockIdx.x; c < spans.start[spans.count]; c += gridDim.x) {
     while (c >= spans.start[span + 1]) ++span;
     const int chunk = c - spans.start[span];
-    switch (spans.type[span]) {
+    const long n = spans.n4t[span] >> 2;
+    switch (spans.n4t[span] & 3) {
       case kF32:
-        sum += chunk_squares<F32>(spans.ptr[span], chunk, spans.n[span]);
+        sum += chunk_squares<F32>(spans.ptr[span], chunk, n);
         break;
       case kBF16:
-        sum += chunk_squares<BF16>(spans.ptr[span], chunk, spans.n[span]);
+        sum += chunk_squares<BF16>(spans.ptr[span], chunk, n);
         break;
       case kF16:
-        sum += chunk_squares<F16>(spans.ptr[span], chunk, spans.n[span]);
+        sum += chunk_squares<F16>(spans.ptr[span], chunk, n);
         break;
     }
   }

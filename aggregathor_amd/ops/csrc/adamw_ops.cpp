@@ -448,14 +448,14 @@ Tensor grad_norm(pybind11::handle given_list) {
       const int last = s.count - 1;
       // Tensors that lie back to back, as views into a flat gradient do, are
       // one span: fewer partly filled chunks, and hardly any search.
-      if (ptr == end && type == s.type[last]) {
-        const int64_t all = s.n[last] + n;
+      if (ptr == end && type == (int)(s.n4t[last] & 3)) {
+        const int64_t all = (s.n4t[last] >> 2) + n;
         const int64_t chunks = (all * t.element_size() +
                                 adamw::kNormChunkBytes - 1) /
                                adamw::kNormChunkBytes;
         TORCH_CHECK(s.start[last] + chunks <= INT32_MAX,
                     "grad_norm: too many elements");
-        s.n[last] = all;
+        s.n4t[last] = 4 * all + type;
         s.start[last + 1] = (int)(s.start[last] + chunks);
         end = ptr + n * t.element_size();
         continue;
@@ -474,8 +474,7 @@ Tensor grad_norm(pybind11::handle given_list) {
     TORCH_CHECK(s.start[i] + chunks <= INT32_MAX,
                 "grad_norm: too many elements");
     s.ptr[i] = ptr;
-    s.n[i] = n;
-    s.type[i] = type;
+    s.n4t[i] = 4 * n + type;
     s.start[i + 1] = (int)(s.start[i] + chunks);
     end = ptr + n * t.element_size();
   }
