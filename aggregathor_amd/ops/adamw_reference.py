@@ -5,6 +5,8 @@ States are computed in the kernels' order, one rounding an operation, so that
 they come out the same bit by bit.
 """
 
+import bisect
+
 import torch
 
 GROUP = 32
@@ -206,12 +208,14 @@ class Plan:
         ranges = sorted(x for x in map(_range, written) if x)
         _check(all(a[1] <= b[0] for a, b in zip(ranges, ranges[1:])),
                "parameters, states and steps share memory")
-        self.ranges = ranges
+        self.ranges, self.ends = ranges, [hi for _, hi in ranges]
 
     def _check_apart(self, t, what):
         r = _range(t)
-        _check(r is None or all(r[1] <= lo or hi <= r[0]
-                                for lo, hi in self.ranges),
+        # The first range that ends behind the tensor's begin.
+        i = 0 if r is None else bisect.bisect_right(self.ends, r[0])
+        _check(r is None or i == len(self.ranges)
+               or r[1] <= self.ranges[i][0],
                f"{what} shares memory with a parameter or state")
 
     @torch.no_grad()
