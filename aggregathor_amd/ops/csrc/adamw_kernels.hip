@@ -383,7 +383,12 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
   const Global<uint8_t> r8s = (Global<uint8_t>)w.rs;
   const int n = w.left;
 
-  // All loads first: they are on their way while the step is counted.
+  // The count first, then all loads of data: loads come back in order, so the
+  // wait for the count leaves the others on their way. (With the count last
+  // VGG-16, clipped, took 705 us instead of 700, ResNet-50 116.2 instead of
+  // 115.5.)
+  int count = __hip_atomic_load(steps + w.tensor, __ATOMIC_RELAXED,
+                                __HIP_MEMORY_SCOPE_AGENT);
   typename P::Quad pq[Quads];
   typename G::Quad gq[Quads];
   f32x4 mq[Quads], vq[Quads];
@@ -403,11 +408,13 @@ __device__ __forceinline__ void update_chunk(const Work& w, const void* grad,
     gq[q] = load4<Full, G>(g_at, i, n);
     pq[q] = load4<Full, P>(param, i, n);
   }
-  const int step = __builtin_amdgcn_readfirstlane(
-      __hip_atomic_load(steps + w.tensor, __ATOMIC_RELAXED,
-                        __HIP_MEMORY_SCOPE_AGENT) + 1);
+  // A barrier waits for no load, and the one behind the arrival that says "read"
+  // would write the count under a wave whose load is still on its way. So each
+  // wave has it in a register before the barrier: this use is where it waits.
+  asm volatile("" : "+v"(count) : : "memory");
   __syncthreads();  // all four waves have read it
   if (threadIdx.x == 0) arrived = arrive(tickets);
+  const int step = __builtin_amdgcn_readfirstlane(count + 1);
   const Common k = common(s, w.key, (uint32_t)step);
 
 #pragma unroll

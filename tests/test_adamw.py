@@ -6,6 +6,8 @@ import io
 import math
 import os
 import pathlib
+import re
+import shutil
 import subprocess
 import sys
 
@@ -16,6 +18,7 @@ import adamw_oracle as oracle
 from aggregathor_amd import ops
 from aggregathor_amd.graph import Engine, build_optimizer
 from aggregathor_amd.ops import adamw_reference as R
+from aggregathor_amd.ops import build as ops_build
 from aggregathor_amd.optim import AdamW
 from aggregathor_amd.parallel import WorkerGroup
 from aggregathor_amd import experiments, tools
@@ -584,3 +587,95 @@ def test_ranks_stay_alike(tmp_path, bits):
     for a, b in zip(one, two):
         assert len(a) == len(b) == (4 if bits == 32 else 6)
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ---------------------------------------------------------------------------- #
+# The kernels' code
+
+
+def _waits(lines):
+    """For each barrier of a kernel's assembly: whether all loads of the step
+    count (the agent-scope ones) that reach it are waited for, or None where
+    none reaches it. Loads come back in order, so with `s_waitcnt vmcnt(n)` a
+    load is there once n or more others have been issued behind it."""
+    blocks, name = {"": []}, ""
+    follows = {}
+    for line in lines:
+        line = line.split(";")[0].strip()
+        if re.match(r"\.LBB\w+:", line):
+            previous, name = name, line[:-1]
+            blocks[name] = []
+            follows.setdefault(previous, set()).add(name)
+        elif line and not line.startswith("."):
+            blocks[name].append(line)
+            if line.startswith(("s_cbranch", "s_branch")):
+                follows.setdefault(name, set()).add(line.split()[1])
+                # What stands behind a branch is a block of its own.
+                previous, name = name, f"{name}+{len(blocks)}"
+                blocks[name] = []
+                if line.startswith("s_cbranch"):
+                    follows[previous].add(name)
+            elif line.startswith("s_endpgm"):
+                name = f"{name}+{len(blocks)}"
+                blocks[name] = []
+    # State: how many others have been issued since (the fewest on any way
+    # here), -1 for one that is there, None before it.
+    states, barriers, todo = {"": {None}}, {}, [""]
+    while todo:
+        at = todo.pop()
+        out = set()
+        for state in states[at]:
+            for k, line in enumerate(blocks[at]):
+                wait = re.search(r"vmcnt\((\d+)\)", line)
+                if re.match(r"global_load_dword v\d+, .* sc1", line):
+                    state = 0
+                elif re.match(r"(global|buffer|flat)_", line):
+                    state = min(state + 1, 64) if state not in (None, -1) \
+                        else state
+                elif line.startswith("s_waitcnt") and wait and \
+                        state not in (None, -1) and int(wait[1]) <= state:
+                    state = -1
+                elif line.startswith("s_barrier"):
+                    barriers.setdefault((at, k), set()).add(state)
+            out.add(state)
+        for to in follows.get(at, ()):
+            if not out <= states.setdefault(to, set()):
+                states[to] |= out
+                todo.append(to)
+    return [None if s == {None} else s == {-1} for s in barriers.values()]
+
+
+def test_waits_are_seen():
+    # The reading of the assembly, on the two ways that a load may be left.
+    def kernel(*wait):
+        return ["s_cbranch_scc0 .LBB0_2", ".LBB0_1:",
+                "global_load_dword v1, v2, s[4:5] sc1",
+                "global_load_dwordx4 v[4:7], v[8:9], off nt",
+                "s_branch .LBB0_3", ".LBB0_2:",
+                "global_load_dword v1, v2, s[4:5] sc1",
+                "global_load_dwordx4 v[4:7], v[8:9], off nt",
+                "global_load_dwordx4 v[4:7], v[8:9], off nt",
+                ".LBB0_3:", *wait, "s_barrier", "s_waitcnt vmcnt(0)",
+                "s_endpgm"]
+    assert _waits(kernel("s_waitcnt vmcnt(1)")) == [True]
+    assert _waits(kernel("s_waitcnt vmcnt(2)")) == [False]
+    assert _waits(kernel()) == [False]
+    assert _waits(["s_barrier", "s_endpgm"]) == [None]
+
+
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="needs hipcc")
+def test_step_counts_are_read_before_the_barrier(tmp_path):
+    # Behind the barrier a workgroup says that it has read the count, and the
+    # last to say so writes it: a wave's load that the barrier does not find
+    # waited for might get the next step's.
+    out = tmp_path / "adamw.s"
+    subprocess.run(["hipcc", "-S", "--cuda-device-only",
+                    *ops_build._compile_flags(),
+                    str(ops_build.CSRC / "adamw_kernels.hip"), "-o", str(out)],
+                   check=True, stderr=subprocess.DEVNULL)
+    kernels = re.findall(r"^(\S*update_kernel\S*):(.*?)^\.Lfunc_end",
+                         out.read_text(), re.M | re.S)
+    assert len(kernels) == 3
+    for name, text in kernels:
+        found = _waits(text.splitlines())
+        assert found and all(found), f"{name}: {found}"
