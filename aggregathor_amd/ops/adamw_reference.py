@@ -169,6 +169,19 @@ class Plan:
     def __init__(self, bits, params, m, ms, r, rs, steps, seed):
         self.bits, self.seed, self.steps = bits, seed, steps
         self.params, self.m, self.ms, self.r, self.rs = params, m, ms, r, rs
+        self._lay_out()
+
+    def _places(self):
+        """Where the plan's tensors lie, and how. (What they were laid out
+        with is out of date once one has got other memory: `param.data = ...`,
+        or a module moved.)"""
+        return [(t.data_ptr(), t.shape, t.stride(), t.dtype, t.device)
+                for t in (self.steps, *self.params, *self.m, *self.ms,
+                          *self.r, *self.rs)]
+
+    def _lay_out(self):
+        bits, steps = self.bits, self.steps
+        params, m, ms, r, rs = self.params, self.m, self.ms, self.r, self.rs
         count, device = len(params), params[0].device
         _check(len(m) == len(r) == count and
                (bits == 32 or len(ms) == len(rs) == count),
@@ -209,6 +222,7 @@ class Plan:
         _check(all(a[1] <= b[0] for a, b in zip(ranges, ranges[1:])),
                "parameters, states and steps share memory")
         self.ranges, self.ends = ranges, [hi for _, hi in ranges]
+        self.places = self._places()
 
     def _check_apart(self, t, what):
         r = _range(t)
@@ -224,6 +238,8 @@ class Plan:
         device = self.params[0].device
         _check(len(grads) == len(self.params), f"{len(self.params)} "
                f"parameters, but {len(grads)} gradients")
+        if self._places() != self.places:
+            self._lay_out()
         clip = None
         if norm is not None:
             _check(norm.device == device and norm.numel() == 1

@@ -327,6 +327,54 @@ def test_step_refuses_what_it_writes_as_input():
                        norm=args[2][0][5], max_norm=1.)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_moved(bits):
+    args, want = (_plan_args(bits=bits) for _ in range(2))
+    make = ops.adamw_plan if bits == 32 else ops.adamw8_plan
+    plan, still = make(*args), make(*want)
+    for _ in range(3):
+        args[0][0].data = args[0][0].data.clone()
+        for one in (plan, still):
+            ops.adamw_step(one, [torch.arange(40.)], lr=0.1)
+    assert torch.equal(args[0][0], want[0][0])
+    # What the new memory holds is not its gradient or its norm.
+    for change in (lambda new: dict(grads=[new]),
+                   lambda new: dict(norm=new[3], max_norm=1.)):
+        args[0][0].data = new = torch.ones(40)
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ops.adamw_step(plan, **{"grads": [torch.ones(40)], "lr": 0.1,
+                                    **change(new)})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_in_another_order_are_refused(bits):
+    # Their states stay in the old one: elements would meet others' states.
+    p = torch.randn(4, 3, 5, 5)
+    state = (ops.adamw8_state(p) if bits == 8 else
+             [torch.zeros_like(p) for _ in range(2)])
+    make = ops.adamw_plan if bits == 32 else ops.adamw8_plan
+    plan = make([p], *[[x] for x in state], _steps(0))
+    ops.adamw_step(plan, [torch.ones(4, 3, 5, 5)], lr=0.1)
+    p.data = p.data.to(memory_format=torch.channels_last)
+    before = p.clone()
+    with pytest.raises(RuntimeError, match="strides"):
+        ops.adamw_step(plan, [torch.ones(4, 3, 5, 5)], lr=0.1)
+    assert torch.equal(p, before)
+
+
+def test_parameters_that_moved_into_gaps_are_refused():
+    args = _plan_args(n=4, bits=32)
+    plan = ops.adamw_plan(*args)
+    whole = torch.arange(8.)
+    args[0][0].data = whole[::2]
+    with pytest.raises(RuntimeError, match="fill its memory"):
+        ops.adamw_step(plan, [torch.ones(4)], lr=0.1)
+    assert torch.equal(whole, torch.arange(8.)) and int(args[3]) == 0
+    args[0][0].data = torch.ones(3)
+    with pytest.raises(RuntimeError):
+        ops.adamw_step(plan, [torch.ones(3)], lr=0.1)
+
+
 def test_16_bit_parameters_refuse_other_gradients():
     p = torch.zeros(8, dtype=torch.bfloat16)
     plan = ops.adamw_plan([p], [torch.zeros(8)], [torch.zeros(8)], _steps(0))
