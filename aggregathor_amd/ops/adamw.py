@@ -55,7 +55,9 @@ def _ext(tensor):
 def grad_norm(grads):
     """L2 norm over all elements of a tensor, or of all tensors of a list, as one
     fp32 number on their device (nothing waits for it). Squares are summed in 64
-    bits, in an order that the tensors' sizes and places alone set."""
+    bits, in an order that the tensors' sizes and places alone set. It is not
+    differentiable: tensors that need a gradient are refused, but under
+    ``torch.no_grad()``."""
     if isinstance(grads, torch.Tensor):
         grads = (grads,)
     elif not isinstance(grads, (list, tuple)):

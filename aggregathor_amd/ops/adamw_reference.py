@@ -21,6 +21,9 @@ def grad_norm(grads):
         if g.dtype not in _TYPES:
             raise RuntimeError("grad_norm: expected fp32, bf16 or fp16, got "
                                f"{g.dtype}")
+        if g.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("grad_norm: has no gradient of its own; detach "
+                               "the tensors or call it under torch.no_grad()")
     return torch.stack([g.double().square().sum()
                         for g in grads]).sum().sqrt().float()
 

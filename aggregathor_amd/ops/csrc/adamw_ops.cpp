@@ -9,6 +9,7 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -430,11 +431,15 @@ Tensor grad_norm(pybind11::handle given_list) {
   std::vector<Tensor> held;
   held.reserve(tensors.size());
   const char* end = nullptr;  // of the last span
+  const bool differentiable = c10::GradMode::is_enabled();
   for (const Tensor* each : tensors) {
     const Tensor& given = *each;
     TORCH_CHECK(given.layout() == torch::kStrided && given.device() == device,
                 "grad_norm: expected dense tensors on one device");
     const int type = dtype_of(given, "grad_norm");
+    TORCH_CHECK(!differentiable || !given.requires_grad(),
+                "grad_norm: has no gradient of its own; detach the tensors or "
+                "call it under torch.no_grad()");
     int64_t n = given.numel();
     if (n == 0) continue;
     // The order of the elements does not matter, only that there are no gaps.

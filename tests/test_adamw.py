@@ -390,6 +390,17 @@ def test_grad_norm_refuses():
             ops.grad_norm(bad)
 
 
+def test_grad_norm_refuses_to_lose_a_gradient():
+    x = torch.ones(4, requires_grad=True)
+    for tensors in ([x], [torch.ones(3), x * 2]):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            ops.grad_norm(tensors)
+    with torch.no_grad():
+        assert float(ops.grad_norm(x)) == 2
+    assert float(ops.grad_norm(x.detach())) == 2
+    assert not ops.grad_norm(torch.ones(3)).requires_grad
+
+
 # ---------------------------------------------------------------------------- #
 # Optimizer
 

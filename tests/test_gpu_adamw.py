@@ -120,6 +120,17 @@ def test_grad_norm_extremes():
     assert float(ops.grad_norm([three] * 4)) == 6
 
 
+def test_grad_norm_refuses_to_lose_a_gradient():
+    x = torch.ones(4, device="cuda", requires_grad=True)
+    for tensors in ([x], [torch.ones(3, device="cuda"), x * 2]):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            ops.grad_norm(tensors)
+    with torch.no_grad():
+        assert float(ops.grad_norm(x)) == 2
+    assert float(ops.grad_norm(x.detach())) == 2
+    assert not ops.grad_norm(torch.ones(3, device="cuda")).requires_grad
+
+
 def test_grad_norm_large():
     # Past 2^32 bytes, and past 2^31 elements in bf16.
     n = (1 << 31) + 4097
