@@ -179,7 +179,9 @@ class AdamW(torch.optim.Optimizer):
         if missing:
             raise ValueError("loaded state dict lacks " + ", ".join(
                 sorted(missing)) + f" of a state of {bits} bits")
-        out = {"step": torch.as_tensor(state["step"]).to(torch.int32)}
+        # A copy: the state may be another optimizer's, which goes on.
+        out = {"step": torch.as_tensor(state["step"]).to(torch.int32,
+                                                         copy=True)}
         names = _STATES[32] if bits == 32 else ("exp_avg", "exp_avg_root")
         for name in names:
             if state[name].shape != p.shape:

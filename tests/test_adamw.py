@@ -550,6 +550,21 @@ def test_loading_does_not_stretch_states():
         AdamW(model.parameters()).load_state_dict(state)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loading_shares_nothing(bits):
+    first, second = _model(), _model()
+    opt = AdamW(first.parameters(), state_bits=bits)
+    _train(first, opt, 2)
+    second.load_state_dict(first.state_dict())
+    opt2 = AdamW(second.parameters(), state_bits=bits)
+    opt2.load_state_dict(opt.state_dict())
+    _train(first, opt, 3, seed=1)  # while the other waits
+    _train(second, opt2, 3, seed=1)
+    assert int(opt2.state[next(second.parameters())]["step"]) == 5
+    for p, q in zip(first.parameters(), second.parameters()):
+        assert torch.equal(p, q)
+
+
 def test_values_refuse():
     codes, scales, *_ = ops.adamw8_state(torch.zeros(100))
     assert torch.equal(ops.adamw8_values(codes, scales), torch.zeros(100))
