@@ -34,7 +34,8 @@ class AdamW(torch.optim.Optimizer):
     A parameter without a gradient is left out of the step, its step count too.
     Each parameter's ``state`` holds ``step`` and the state tensors; they may be
     changed in place, and replaced by :meth:`load_state_dict`, which also takes
-    the state of a ``torch.optim.Adam`` or ``AdamW`` (32 bits).
+    the state of a ``torch.optim.AdamW``, or of an ``Adam`` without weight decay
+    (32 bits).
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -158,6 +159,13 @@ class AdamW(torch.optim.Optimizer):
                 if group.get(other):
                     raise ValueError(f"loaded state dict is of a step with "
                                      f"{other}, which this optimizer has not")
+            # torch's Adam adds its decay to the gradient (and says so; what is
+            # no Adam at all has no betas).
+            if given.get("weight_decay") and "state_bits" not in given and \
+                    not given.get("decoupled_weight_decay", "betas" in given):
+                raise ValueError("loaded state dict is of a step whose weight "
+                                 "decay goes through the gradient; here it is "
+                                 "decoupled")
             groups.append(group)
         saved = [i for group in groups for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]

@@ -565,6 +565,29 @@ def test_loading_shares_nothing(bits):
         assert torch.equal(p, q)
 
 
+def test_loads_no_decay_that_is_not_decoupled():
+    model = _model()
+    for other in (torch.optim.Adam, torch.optim.SGD):
+        opt = other(model.parameters(), lr=0.1, weight_decay=0.1)
+        with pytest.raises(ValueError, match="decoupled"):
+            AdamW(model.parameters()).load_state_dict(opt.state_dict())
+    other = AdamW(model.parameters(), weight_decay=0.3)
+    other.load_state_dict(torch.optim.Rprop(model.parameters()).state_dict())
+    assert other.param_groups[0]["weight_decay"] == 0.3  # it has none to give
+    for opt in (torch.optim.AdamW(model.parameters(), weight_decay=0.1),
+                torch.optim.Adam(model.parameters())):
+        _train(model, opt, 1)
+        mine = AdamW(model.parameters())
+        mine.load_state_dict(opt.state_dict())
+        decay = opt.param_groups[0]["weight_decay"]
+        assert mine.param_groups[0]["weight_decay"] == decay
+        # From then on it is this optimizer's, with the decay that it has.
+        mine.param_groups[0]["weight_decay"] = 0.2
+        again = AdamW(model.parameters())
+        again.load_state_dict(mine.state_dict())
+        assert again.param_groups[0]["weight_decay"] == 0.2
+
+
 def test_values_refuse():
     codes, scales, *_ = ops.adamw8_state(torch.zeros(100))
     assert torch.equal(ops.adamw8_values(codes, scales), torch.zeros(100))
