@@ -148,7 +148,29 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Load what :meth:`state_dict` gave. (The base class would cast every
-        state to its parameter's type.)"""
+        state to its parameter's type: it gets none to cast.)"""
+        states = {}
+
+        def take(_, given):  # behind the caller's hooks, which may change it
+            groups, found = self._readable(given)
+            states.update(found)
+            return {"state": {}, "param_groups": groups}
+
+        def keep(_):  # ahead of the caller's hooks, which may look at it
+            self.state.update(states)
+            self._plans = None
+
+        hooks = (self.register_load_state_dict_pre_hook(take),
+                 self.register_load_state_dict_post_hook(keep, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _readable(self, state_dict):
+        """The groups and states of a state dict, where the optimizer can go on
+        with them."""
         groups = []
         for given in state_dict["param_groups"]:
             group = {**self.defaults, **given}
@@ -177,9 +199,7 @@ class AdamW(torch.optim.Optimizer):
         states = {p: self._loaded(state_dict["state"][i], p, b)
                   for i, p, b in zip(saved, params, bits)
                   if i in state_dict["state"]}
-        super().load_state_dict({"state": {}, "param_groups": groups})
-        self.state.update(states)
-        self._plans = None
+        return groups, states
 
     @staticmethod
     def _loaded(state, p, bits):

@@ -588,6 +588,39 @@ def test_loads_no_decay_that_is_not_decoupled():
         assert again.param_groups[0]["weight_decay"] == 0.2
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_hooks_see_the_states(bits):
+    model = _model()
+    opt = AdamW(model.parameters(), state_bits=bits)
+    _train(model, opt, 3)
+    saved, seen = opt.state_dict(), []
+
+    def before(_, given):
+        seen.append(sorted(given["state"]))
+        states = {i: {**s, "step": torch.tensor(7)}
+                  for i, s in given["state"].items()}
+        return {**given, "state": states}
+
+    def after(optimizer):
+        seen.append([int(optimizer.state[p]["step"])
+                     for p in model.parameters()])
+
+    opt2 = AdamW(model.parameters())
+    opt2.register_load_state_dict_pre_hook(before)
+    opt2.register_load_state_dict_post_hook(after)
+    for _ in range(2):
+        opt2.load_state_dict(saved)
+    assert seen == [[0, 1, 2, 3], [7] * 4] * 2
+    _train(model, opt2, 1)
+    assert int(opt2.state[next(model.parameters())]["step"]) == 8
+    # What is refused leaves the optimizer as it was.
+    saved["param_groups"][0]["state_bits"] = 40 - bits
+    with pytest.raises(ValueError):
+        opt2.load_state_dict(saved)
+    assert opt2.param_groups[0]["state_bits"] == bits
+    assert int(opt2.state[next(model.parameters())]["step"]) == 8
+
+
 def test_values_refuse():
     codes, scales, *_ = ops.adamw8_state(torch.zeros(100))
     assert torch.equal(ops.adamw8_values(codes, scales), torch.zeros(100))
