@@ -228,6 +228,10 @@ class AdamW(torch.optim.Optimizer):
             if codes.dtype != torch.float8_e4m3fn or \
                     scales.dtype != torch.float8_e8m0fnu:
                 raise ValueError(f"loaded {name} is no 8-bit state")
+            if scales.shape != (-(-codes.numel() // reference.GROUP),):
+                raise ValueError(f"loaded {name}_scale has the shape "
+                                 f"{tuple(scales.shape)}, not one element for "
+                                 f"{reference.GROUP} of {name}")
             if reference._same_layout(codes, p):
                 codes, scales = codes.clone(), scales.clone()
             else:

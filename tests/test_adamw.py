@@ -621,6 +621,17 @@ def test_load_hooks_see_the_states(bits):
     assert int(opt2.state[next(model.parameters())]["step"]) == 8
 
 
+def test_loading_takes_scales_of_the_right_number():
+    model = _model()
+    opt = AdamW(model.parameters(), state_bits=8)
+    _train(model, opt, 1)
+    for name in ("exp_avg_scale", "exp_avg_root_scale"):
+        saved = copy.deepcopy(opt.state_dict())
+        saved["state"][2][name] = saved["state"][2][name][1:]
+        with pytest.raises(ValueError, match=name):
+            AdamW(model.parameters()).load_state_dict(saved)
+
+
 def test_values_refuse():
     codes, scales, *_ = ops.adamw8_state(torch.zeros(100))
     assert torch.equal(ops.adamw8_values(codes, scales), torch.zeros(100))
