@@ -120,6 +120,23 @@ def adamw8_values(codes, scales):
     return reference.values8(codes, scales)
 
 
+def out_of_range(lr, beta1, beta2, eps, weight_decay, max_norm=None):
+    """What is wrong with the settings of a step, None where nothing is."""
+    for name, value, ok in (
+            ("lr", lr, 0. <= lr < math.inf),
+            ("beta1", beta1, 0. <= beta1 < 1.),
+            ("beta2", beta2, 0. <= beta2 < 1.),
+            # Normal numbers, also behind a division: the kernels' reciprocal
+            # takes others for zero.
+            ("eps", eps, 1.2e-38 <= eps <= 1e30),
+            ("weight_decay", weight_decay, 0. <= weight_decay < math.inf),
+            ("max_norm", max_norm,
+             max_norm is None or 1.2e-38 <= max_norm < 3e38)):
+        if not ok:
+            return f"{name} = {value} is out of range"
+    return None
+
+
 def adamw_step(plan, grads, lr, beta1=0.9, beta2=0.999, eps=1e-8,
                weight_decay=0.01, norm=None, max_norm=None):
     """One AdamW step over all tensors of a plan, in place.
@@ -139,20 +156,13 @@ def adamw_step(plan, grads, lr, beta1=0.9, beta2=0.999, eps=1e-8,
     Work on a plan from two streams has to be ordered by the caller, as for any
     tensors that are updated in place.
     """
-    for name, value, ok in (
-            ("lr", lr, 0. <= lr < math.inf),
-            ("beta1", beta1, 0. <= beta1 < 1.),
-            ("beta2", beta2, 0. <= beta2 < 1.),
-            ("eps", eps, 1.2e-38 <= eps <= 1e30),
-            ("weight_decay", weight_decay, 0. <= weight_decay < math.inf)):
-        if not ok:
-            raise RuntimeError(f"adamw: {name} = {value} is out of range")
+    refusal = out_of_range(lr, beta1, beta2, eps, weight_decay, max_norm)
+    if refusal:
+        raise RuntimeError("adamw: " + refusal)
     if (norm is None) != (max_norm is None):
         raise RuntimeError("adamw: norm and max_norm belong together")
     if max_norm is None:
         max_norm = 1.
-    elif not 1.2e-38 <= max_norm < 3e38:
-        raise RuntimeError(f"adamw: max_norm = {max_norm} is out of range")
     if not isinstance(grads, (list, tuple)):
         grads = list(grads)
     plan.step(grads, lr, beta1, beta2, eps, weight_decay, norm, max_norm)

@@ -14,6 +14,7 @@ import torch
 
 from . import ops, tools
 from .ops import adamw_reference as reference
+from .ops.adamw import out_of_range
 
 _STATES = {32: ("exp_avg", "exp_avg_sq"),
            8: ("exp_avg", "exp_avg_scale", "exp_avg_root",
@@ -41,9 +42,6 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
                  weight_decay=1e-2, state_bits=32, max_norm=None,
                  rounding_seed=0):
-        if max_norm is not None and not max_norm > 0:
-            raise tools.UserException(
-                f"adamw: expected a positive norm to clip to, got {max_norm}")
         self.max_norm = max_norm
         self.rounding_seed = rounding_seed
         self._plans = None
@@ -53,7 +51,15 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        self._check_bits(self.param_groups[-1])
+        group = self.param_groups[-1]
+        try:
+            self._check_bits(group)
+            refusal = self._refusal(group)
+            if refusal:
+                raise tools.UserException("adamw: " + refusal)
+        except Exception:
+            self.param_groups.pop()
+            raise
         self._plans = None
 
     def __setstate__(self, state):
@@ -64,6 +70,11 @@ class AdamW(torch.optim.Optimizer):
         # Plans are laid out anew where the optimizer is copied to.
         return dict(super().__getstate__(), max_norm=self.max_norm,
                     rounding_seed=self.rounding_seed)
+
+    def _refusal(self, group):
+        """What is wrong with a group's settings."""
+        return out_of_range(float(group["lr"]), *group["betas"], group["eps"],
+                            group["weight_decay"], self.max_norm)
 
     @staticmethod
     def _check_bits(group):
@@ -177,6 +188,9 @@ class AdamW(torch.optim.Optimizer):
             if state_dict["state"] and "state_bits" not in given:
                 group["state_bits"] = 32  # torch's own
             self._check_bits(group)
+            refusal = self._refusal(group)
+            if refusal:
+                raise ValueError("loaded state dict: " + refusal)
             for other in ("amsgrad", "maximize"):
                 if group.get(other):
                     raise ValueError(f"loaded state dict is of a step with "

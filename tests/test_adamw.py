@@ -632,6 +632,28 @@ def test_loading_takes_scales_of_the_right_number():
             AdamW(model.parameters()).load_state_dict(saved)
 
 
+@pytest.mark.parametrize("setting", [
+    dict(lr=-1.), dict(lr=math.nan), dict(betas=(1., 0.9)),
+    dict(betas=(0.9, -0.1)), dict(eps=0.), dict(weight_decay=-1.),
+    dict(max_norm=-1.), dict(max_norm=math.inf), dict(max_norm=1e-40),
+    dict(max_norm=math.nan)])
+def test_settings_that_no_step_takes_are_refused_at_once(setting):
+    model = _model()
+    with pytest.raises(tools.UserException):
+        AdamW(model.parameters(), **setting)
+    if "max_norm" in setting:
+        return
+    first, *others = model.parameters()
+    opt = AdamW([first])
+    with pytest.raises(tools.UserException):
+        opt.add_param_group({"params": others, **setting})
+    assert len(opt.param_groups) == 1
+    saved = AdamW(model.parameters()).state_dict()
+    saved["param_groups"][0].update(setting)
+    with pytest.raises(ValueError, match="out of range"):
+        AdamW(model.parameters()).load_state_dict(saved)
+
+
 def test_values_refuse():
     codes, scales, *_ = ops.adamw8_state(torch.zeros(100))
     assert torch.equal(ops.adamw8_values(codes, scales), torch.zeros(100))
