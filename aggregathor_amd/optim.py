@@ -10,6 +10,9 @@ The result is a function of parameters, gradients and states alone, bit by bit:
 ranks that hold the same aggregated gradient keep the same parameters.
 """
 
+from itertools import chain, starmap, zip_longest
+from operator import is_
+
 import torch
 
 from . import ops, tools
@@ -19,6 +22,20 @@ from .ops.adamw import out_of_range
 _STATES = {32: ("exp_avg", "exp_avg_sq"),
            8: ("exp_avg", "exp_avg_scale", "exp_avg_root",
                "exp_avg_root_scale")}
+
+
+class _Held:
+    """A plan, and the parameters and states that it is over."""
+
+    def __init__(self, group, params, plan, tensors):
+        self.group, self.params, self.plan = group, params, plan
+        self._tensors = tensors  # of each parameter's state, by name
+
+    def holds(self, states):
+        """Whether the states are still those."""
+        return all(states[p].get(name) is tensor
+                   for p, tensors in zip(self.params, self._tensors)
+                   for name, tensor in tensors.items())
 
 
 class AdamW(torch.optim.Optimizer):
@@ -34,9 +51,9 @@ class AdamW(torch.optim.Optimizer):
 
     A parameter without a gradient is left out of the step, its step count too.
     Each parameter's ``state`` holds ``step`` and the state tensors; they may be
-    changed in place, and replaced by :meth:`load_state_dict`, which also takes
-    the state of a ``torch.optim.AdamW``, or of an ``Adam`` without weight decay
-    (32 bits).
+    changed in place, replaced, or cleared (the next step starts from zero
+    there). :meth:`load_state_dict` replaces them; it also takes the state of a
+    ``torch.optim.AdamW``, or of an ``Adam`` without weight decay (32 bits).
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -44,7 +61,7 @@ class AdamW(torch.optim.Optimizer):
                  rounding_seed=0):
         self.max_norm = max_norm
         self.rounding_seed = rounding_seed
-        self._plans = None
+        self._plans, self._laid_out = [], False
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps,
                                       weight_decay=weight_decay,
                                       state_bits=state_bits))
@@ -60,11 +77,11 @@ class AdamW(torch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
-        self._plans = None
+        self._laid_out = False
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans = None
+        self._plans, self._laid_out = [], False
 
     def __getstate__(self):
         # Plans are laid out anew where the optimizer is copied to.
@@ -85,51 +102,67 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ #
 
     def _lay_out(self):
-        """Make the states that are missing, and a plan for each group (and
-        each device of its parameters)."""
-        if torch.cuda.is_available() and \
-                torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("adamw: run a step before the capture, so that "
-                               "the states and plans are there")
-        plans, first_steps = [], []
+        """A plan for each group (and each device of its parameters) where there
+        is none over its states, and the states that are missing."""
+        self._laid_out = False
+        self._plans = [plan for plan in self._plans if plan.holds(self.state)]
+        held = {p for plan in self._plans for p in plan.params}
         for index, group in enumerate(self.param_groups):
-            self._check_bits(group)
-            bits = group["state_bits"]
             by_device = {}
             for p in group["params"]:
-                by_device.setdefault(p.device, []).append(p)
+                if p not in held:
+                    by_device.setdefault(p.device, []).append(p)
             for device, params in by_device.items():
-                steps = torch.zeros(len(params), dtype=torch.int32,
-                                    device=device)
-                columns = [[] for _ in _STATES[bits]]
-                for i, p in enumerate(params):
-                    state = self.state[p]
-                    if "step" in state:
-                        steps[i] = state["step"]
-                    else:
-                        fresh = (ops.adamw8_state(p) if bits == 8 else
-                                 [torch.zeros_like(p, dtype=torch.float32,
-                                                   requires_grad=False)
-                                  for _ in range(2)])
-                        state.update(zip(_STATES[bits], fresh))
-                    state["step"] = steps[i]  # a view: the plan counts there
-                    for column, name in zip(columns, _STATES[bits]):
-                        column.append(state[name])
-                if bits == 8:
-                    plan = ops.adamw8_plan(params, *columns, steps,
-                                           seed=self.rounding_seed + index)
-                else:
-                    plan = ops.adamw_plan(params, *columns, steps)
-                plans.append((group, params, plan))
-                first_steps.append(self.state[params[0]]["step"])
-        self._plans, self._first_steps = plans, first_steps
+                if torch.cuda.is_available() and \
+                        torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(
+                        "adamw: run a step before the capture, so that the "
+                        "states and plans are there")
+                self._check_bits(group)
+                self._plans.append(self._plan(group, index, params, device))
+        self._seen = list(self._all_states())
+        self._laid_out = True
 
-    def _state_kept(self):
-        """Whether the plans still hold the state (a user may have cleared it;
-        the first parameter of each tells)."""
-        return all(self.state[params[0]].get("step") is first
-                   for (_, params, _), first in zip(self._plans,
-                                                    self._first_steps))
+    def _all_states(self):
+        return chain.from_iterable(map(dict.values, self.state.values()))
+
+    def _states_kept(self):
+        """Whether all states are what they were (a caller may have cleared or
+        replaced some). Without a lookup by parameter, which hashes it in
+        Python: 161 parameters took 59 us so, and take 17."""
+        return all(starmap(is_, zip_longest(self._all_states(), self._seen,
+                                            fillvalue=self)))
+
+    def _plan(self, group, index, params, device):
+        bits = group["state_bits"]
+        steps = torch.zeros(len(params), dtype=torch.int32, device=device)
+        columns = [[] for _ in _STATES[bits]]
+        for i, p in enumerate(params):
+            state = self.state[p]
+            if "step" in state:
+                missing = set(_STATES[bits]) - set(state)
+                if missing:
+                    raise RuntimeError("adamw: a state lacks " + ", ".join(
+                        sorted(missing)))
+                steps[i] = state["step"]
+            else:
+                fresh = (ops.adamw8_state(p) if bits == 8 else
+                         [torch.zeros_like(p, dtype=torch.float32,
+                                           requires_grad=False)
+                          for _ in range(2)])
+                state.update(zip(_STATES[bits], fresh))
+            state["step"] = steps[i]  # a view: the plan counts there
+            for column, name in zip(columns, _STATES[bits]):
+                column.append(state[name])
+        if bits == 8:
+            plan = ops.adamw8_plan(params, *columns, steps,
+                                   seed=self.rounding_seed + index)
+        else:
+            plan = ops.adamw_plan(params, *columns, steps)
+        names = ("step", *_STATES[bits])
+        return _Held(group, params, plan,
+                     [{name: self.state[p][name] for name in names}
+                      for p in params])
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -138,18 +171,19 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._plans is None or not self._state_kept():
+        if not self._laid_out or not self._states_kept():
             self._lay_out()
-        grads = [[p.grad for p in params] for _, params, _ in self._plans]
+        grads = [[p.grad for p in held.params] for held in self._plans]
         norm = None
         if self.max_norm is not None:
             present = [g for part in grads for g in part if g is not None]
             if not present:
                 return loss
             norm = ops.grad_norm(present)
-        for (group, _, plan), part in zip(self._plans, grads):
+        for held, part in zip(self._plans, grads):
+            group = held.group
             beta1, beta2 = group["betas"]
-            ops.adamw_step(plan, part, lr=float(group["lr"]), beta1=beta1,
+            ops.adamw_step(held.plan, part, lr=float(group["lr"]), beta1=beta1,
                            beta2=beta2, eps=group["eps"],
                            weight_decay=group["weight_decay"], norm=norm,
                            max_norm=self.max_norm)
@@ -169,7 +203,7 @@ class AdamW(torch.optim.Optimizer):
 
         def keep(_):  # ahead of the caller's hooks, which may look at it
             self.state.update(states)
-            self._plans = None
+            self._plans, self._laid_out = [], False
 
         hooks = (self.register_load_state_dict_pre_hook(take),
                  self.register_load_state_dict_post_hook(keep, prepend=True))

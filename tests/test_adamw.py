@@ -700,6 +700,50 @@ def test_groups_with_their_own_settings():
     assert int(opt.state[params[0]]["step"]) == 1
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_that_are_cleared_or_replaced(bits):
+    whole, other = _model(), _model()
+    opt = AdamW(whole.parameters(), state_bits=bits)
+    opt2 = AdamW(other.parameters(), state_bits=bits)
+    for model, optimizer in ((whole, opt), (other, opt2)):
+        _train(model, optimizer, 2)
+    params, params2 = list(whole.parameters()), list(other.parameters())
+    # Through the state and through load_state_dict.
+    names = [k for k in opt.state[params[2]] if k != "step"]
+    replaced = {k: v.clone() for k, v in zip(
+        names, ops.adamw8_state(params[2]) if bits == 8 else
+        [torch.ones_like(params[2]) for _ in range(2)])}
+    del opt.state[params[1]]
+    opt.state[params[2]].update(replaced)
+    opt.state[params[3]]["step"] = 7
+    saved = opt2.state_dict()
+    del saved["state"][1]
+    saved["state"][2].update(replaced)
+    saved["state"][3]["step"] = 7
+    opt2.load_state_dict(saved)
+    for model, optimizer in ((whole, opt), (other, opt2)):
+        _train(model, optimizer, 2, seed=1)
+    for p, q in zip(params, params2):
+        assert torch.equal(p, q)
+        x, y = opt.state[p], opt2.state[q]
+        assert set(x) == set(y) == {"step", *names}
+        assert all(torch.equal(x[k].float(), y[k].float()) for k in x)
+    assert [int(opt.state[p]["step"]) for p in params] == [4, 2, 4, 9]
+    assert sorted(opt.state_dict()["state"]) == [0, 1, 2, 3]
+
+
+def test_states_that_are_incomplete_are_refused():
+    model = _model()
+    opt = AdamW(model.parameters())
+    _train(model, opt, 1)
+    before = [p.detach().clone() for p in model.parameters()]
+    del opt.state[next(model.parameters())]["exp_avg"]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="lacks exp_avg"):
+            opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(before, model.parameters()))
+
+
 def test_registry():
     p = [torch.nn.Parameter(torch.zeros(4))]
     opt = build_optimizer("adamw", ["state-bits:8", "clip-norm:2",
