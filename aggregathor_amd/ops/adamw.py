@@ -68,14 +68,15 @@ def grad_norm(grads):
     return (reference if ext is None else ext).grad_norm(grads)
 
 
-def _plan(bits, params, m, ms, r, rs, steps, seed):
+def _plan(bits, params, m, ms, r, rs, steps, seed, places=None):
     params = list(params)
     if not params:
         raise RuntimeError("adamw: a plan needs a parameter")
     ext = _ext(params[0])
     make = reference.Plan if ext is None else ext.AdamWPlan
+    places = range(len(params)) if places is None else places
     return make(bits, params, list(m), list(ms), list(r), list(rs), steps,
-                int(seed) & 0xFFFFFFFF)
+                int(seed) & 0xFFFFFFFF, [int(i) & 0xFFFFFFFF for i in places])
 
 
 def adamw_plan(params, exp_avgs, exp_avg_sqs, steps):
@@ -92,7 +93,7 @@ def adamw_plan(params, exp_avgs, exp_avg_sqs, steps):
 
 
 def adamw8_plan(params, exp_avgs, exp_avg_scales, exp_avg_roots,
-                exp_avg_root_scales, steps, seed=0):
+                exp_avg_root_scales, steps, seed=0, places=None):
     """A plan over 8-bit states (made by :func:`adamw8_state`).
 
     Args:
@@ -103,9 +104,12 @@ def adamw8_plan(params, exp_avgs, exp_avg_scales, exp_avg_roots,
       exp_avg_root_scales: their scales
       steps:               int32 tensor, as of :func:`adamw_plan`
       seed:                of the rounding (its low 32 bits)
+      places:              of each parameter, the number that stands for it in
+                           the rounding (None: 0, 1, ...); with its own it is
+                           rounded alike in any plan
     """
     return _plan(8, params, exp_avgs, exp_avg_scales, exp_avg_roots,
-                 exp_avg_root_scales, steps, seed)
+                 exp_avg_root_scales, steps, seed, places)
 
 
 def adamw8_state(param):

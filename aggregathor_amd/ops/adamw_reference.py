@@ -169,12 +169,13 @@ def _check(ok, message):
 class Plan:
     """The kernels' plan, in plain PyTorch."""
 
-    def __init__(self, bits, params, m, ms, r, rs, steps, seed):
+    def __init__(self, bits, params, m, ms, r, rs, steps, seed, places):
         self.bits, self.seed, self.steps = bits, seed, steps
+        self.places = places
         self.params, self.m, self.ms, self.r, self.rs = params, m, ms, r, rs
         self._lay_out()
 
-    def _places(self):
+    def _memory(self):
         """Where the plan's tensors lie, and how. (What they were laid out
         with is out of date once one has got other memory: `param.data = ...`,
         or a module moved.)"""
@@ -189,6 +190,8 @@ class Plan:
         _check(len(m) == len(r) == count and
                (bits == 32 or len(ms) == len(rs) == count),
                "as many states as parameters are needed")
+        _check(len(self.places) == count,
+               "as many places as parameters are needed")
         _check(steps.device == device and steps.shape == (count,)
                and steps.is_contiguous() and steps.dtype == torch.int32,
                "steps is a contiguous int32 tensor of one count for each "
@@ -225,7 +228,7 @@ class Plan:
         _check(all(a[1] <= b[0] for a, b in zip(ranges, ranges[1:])),
                "parameters, states and steps share memory")
         self.ranges, self.ends = ranges, [hi for _, hi in ranges]
-        self.places = self._places()
+        self.memory = self._memory()
 
     def _check_apart(self, t, what):
         r = _range(t)
@@ -241,7 +244,7 @@ class Plan:
         device = self.params[0].device
         _check(len(grads) == len(self.params), f"{len(self.params)} "
                f"parameters, but {len(grads)} gradients")
-        if self._places() != self.places:
+        if self._memory() != self.memory:
             self._lay_out()
         clip = None
         if norm is not None:
@@ -297,8 +300,8 @@ class Plan:
             ms.copy_(m)
             rs.copy_(v)
             return
-        bits = random_bits(self.seed, i, int(self.steps[i]), p.numel(),
-                           p.device)
+        bits = random_bits(self.seed, self.places[i], int(self.steps[i]),
+                           p.numel(), p.device)
         for codes, scales, x, of, root_, chance in (
                 (ms, self.ms[i], m, m, False, bits & 0xFFFF),
                 (rs, self.rs[i], root, v, True, bits >> 16)):

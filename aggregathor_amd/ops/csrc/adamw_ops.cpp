@@ -114,7 +114,7 @@ class Plan {
  public:
   Plan(int bits, std::vector<Tensor> params, std::vector<Tensor> m,
        std::vector<Tensor> ms, std::vector<Tensor> r, std::vector<Tensor> rs,
-       Tensor steps, int64_t seed)
+       Tensor steps, int64_t seed, std::vector<int64_t> places)
       : bits_(bits),
         params_(std::move(params)),
         m_(std::move(m)),
@@ -122,7 +122,8 @@ class Plan {
         r_(std::move(r)),
         rs_(std::move(rs)),
         steps_(std::move(steps)),
-        seed_((uint32_t)seed) {
+        seed_((uint32_t)seed),
+        places_(std::move(places)) {
     TORCH_CHECK(bits_ == 8 || bits_ == 32, "adamw: states have 8 or 32 bits");
     TORCH_CHECK(!params_.empty(), "adamw: a plan needs a parameter");
     lay_out();
@@ -271,6 +272,8 @@ class Plan {
                     (bits_ == 32 ||
                      (ms_.size() == count && rs_.size() == count)),
                 "adamw: as many states as parameters are needed");
+    TORCH_CHECK(places_.size() == count,
+                "adamw: as many places as parameters are needed");
     TORCH_CHECK(steps_.device() == device && steps_.dim() == 1 &&
                     steps_.size(0) == (int64_t)count &&
                     steps_.is_contiguous() &&
@@ -303,7 +306,7 @@ class Plan {
       t.p = p.data_ptr();
       t.m = m_[i].data_ptr();
       t.r = r_[i].data_ptr();
-      t.key = mix(seed_ + 0x9E3779B9u * (uint32_t)(i + 1));
+      t.key = mix(seed_ + 0x9E3779B9u * (uint32_t)(places_[i] + 1));
       t.type = dtype_of(p, "adamw: parameter");
       written.push_back(range_of(p));
       written.push_back(range_of(m_[i]));
@@ -385,6 +388,7 @@ class Plan {
   std::vector<Tensor> params_, m_, ms_, r_, rs_;
   Tensor steps_;
   uint32_t seed_;
+  std::vector<int64_t> places_;  // what stands for a tensor in its random bits
   std::vector<adamw::Work> table_;  // each tensor's first
   std::vector<int64_t> work_start_;  // before each tensor's, in device_work_
   int64_t chunk_ = 0;
@@ -516,7 +520,8 @@ void register_adamw(pybind11::module& mod) {
   py::class_<Plan>(mod, "AdamWPlan")
       .def(py::init<int, std::vector<Tensor>, std::vector<Tensor>,
                     std::vector<Tensor>, std::vector<Tensor>,
-                    std::vector<Tensor>, Tensor, int64_t>())
+                    std::vector<Tensor>, Tensor, int64_t,
+                    std::vector<int64_t>>())
       .def("step", &Plan::step);
   mod.def("grad_norm", &grad_norm,
           "L2 norm over all elements of many tensors (gfx950)");

@@ -33,7 +33,7 @@ class _Held:
 
     def holds(self, states):
         """Whether the states are still those."""
-        return all(states[p].get(name) is tensor
+        return all(states.get(p, {}).get(name) is tensor
                    for p, tensors in zip(self.params, self._tensors)
                    for name, tensor in tensors.items())
 
@@ -49,7 +49,8 @@ class AdamW(torch.optim.Optimizer):
                      (None: no clipping; parameters on one device only)
       rounding_seed: of the 8-bit states' rounding
 
-    A parameter without a gradient is left out of the step, its step count too.
+    A parameter without a gradient is left out of the step, its step count too;
+    it has no state before it first has a gradient.
     Each parameter's ``state`` holds ``step`` and the state tensors; they may be
     changed in place, replaced, or cleared (the next step starts from zero
     there). :meth:`load_state_dict` replaces them; it also takes the state of a
@@ -102,16 +103,26 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ #
 
     def _lay_out(self):
-        """A plan for each group (and each device of its parameters) where there
-        is none over its states, and the states that are missing."""
+        """Plans over the parameters that have a gradient or a state, where
+        there is none over their states: one for each group (and each device)
+        and each time that some of its parameters are the first to have one.
+        What a plan holds stays where it is, also for a captured step."""
         self._laid_out = False
         self._plans = [plan for plan in self._plans if plan.holds(self.state)]
         held = {p for plan in self._plans for p in plan.params}
+        waiting = []
         for index, group in enumerate(self.param_groups):
-            by_device = {}
+            by_device, places = {}, {}
             for p in group["params"]:
-                if p not in held:
-                    by_device.setdefault(p.device, []).append(p)
+                # Its number among the group's on its device, whether or not
+                # the others are there.
+                place = places[p.device] = places.get(p.device, -1) + 1
+                if p in held:
+                    continue
+                if p.grad is None and not self.state.get(p):
+                    waiting.append(p)
+                else:
+                    by_device.setdefault(p.device, []).append((place, p))
             for device, params in by_device.items():
                 if torch.cuda.is_available() and \
                         torch.cuda.is_current_stream_capturing():
@@ -119,7 +130,14 @@ class AdamW(torch.optim.Optimizer):
                         "adamw: run a step before the capture, so that the "
                         "states and plans are there")
                 self._check_bits(group)
-                self._plans.append(self._plan(group, index, params, device))
+                self._plans.append(self._plan(group, index, device,
+                                              *zip(*params)))
+        there = [p for plan in self._plans for p in plan.params]
+        held = set(there)
+        self._in_order = all(map(is_, there, (
+            p for group in self.param_groups for p in group["params"]
+            if p in held)))
+        self._waiting = waiting
         self._seen = list(self._all_states())
         self._laid_out = True
 
@@ -133,7 +151,7 @@ class AdamW(torch.optim.Optimizer):
         return all(starmap(is_, zip_longest(self._all_states(), self._seen,
                                             fillvalue=self)))
 
-    def _plan(self, group, index, params, device):
+    def _plan(self, group, index, device, places, params):
         bits = group["state_bits"]
         steps = torch.zeros(len(params), dtype=torch.int32, device=device)
         columns = [[] for _ in _STATES[bits]]
@@ -156,7 +174,8 @@ class AdamW(torch.optim.Optimizer):
                 column.append(state[name])
         if bits == 8:
             plan = ops.adamw8_plan(params, *columns, steps,
-                                   seed=self.rounding_seed + index)
+                                   seed=self.rounding_seed + index,
+                                   places=places)
         else:
             plan = ops.adamw_plan(params, *columns, steps)
         names = ("step", *_STATES[bits])
@@ -171,12 +190,17 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if not self._laid_out or not self._states_kept():
+        if not self._laid_out or not self._states_kept() or any(
+                p.grad is not None for p in self._waiting):
             self._lay_out()
         grads = [[p.grad for p in held.params] for held in self._plans]
         norm = None
         if self.max_norm is not None:
-            present = [g for part in grads for g in part if g is not None]
+            # In the order of the parameters, which the sum's depends on.
+            present = [g for part in (grads if self._in_order else (
+                [p.grad for p in group["params"]]
+                for group in self.param_groups)) for g in part
+                       if g is not None]
             if not present:
                 return loss
             norm = ops.grad_norm(present)
@@ -246,7 +270,7 @@ class AdamW(torch.optim.Optimizer):
                              "parameters than the optimizer")
         states = {p: self._loaded(state_dict["state"][i], p, b)
                   for i, p, b in zip(saved, params, bits)
-                  if i in state_dict["state"]}
+                  if state_dict["state"].get(i)}
         return groups, states
 
     @staticmethod

@@ -285,6 +285,13 @@ def test_plan_refuses(bits, place, value):
         make(*args)
 
 
+def test_plan_refuses_another_number_of_places():
+    for places in ([], [0, 1]):
+        with pytest.raises(RuntimeError, match="places"):
+            ops.adamw8_plan(*_plan_args(), places=places)
+    ops.adamw8_plan(*_plan_args(), places=[3])
+
+
 def test_plan_refuses_shared_memory():
     flat = torch.zeros(100)
     other = lambda: [torch.zeros(40), torch.zeros(40)]  # noqa: E731
@@ -742,6 +749,67 @@ def test_states_that_are_incomplete_are_refused():
         with pytest.raises(RuntimeError, match="lacks exp_avg"):
             opt.step()
     assert all(torch.equal(a, b) for a, b in zip(before, model.parameters()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_only_parameters_with_a_gradient_have_a_state(bits):
+    frozen = torch.nn.Parameter(torch.zeros(9, dtype=torch.float64),
+                                requires_grad=False)
+    late = torch.nn.Parameter(torch.ones(70))
+    model = _model()
+    opt = AdamW([frozen, late, *model.parameters()], state_bits=bits)
+    _train(model, opt, 2)
+    assert not opt.state.get(frozen) and not opt.state.get(late)
+    assert sorted(opt.state_dict()["state"]) == [2, 3, 4, 5]
+    first = opt.state[next(model.parameters())]["step"]
+    late.grad = torch.arange(70.)
+    opt.step()
+    assert int(opt.state[late]["step"]) == 1
+    # What was there has not moved.
+    assert opt.state[next(model.parameters())]["step"] is first
+    assert int(first) == 3 and not opt.state.get(frozen)
+    again = AdamW([frozen, late, *model.parameters()])
+    again.load_state_dict(opt.state_dict())
+    again.step()
+    assert int(again.state[late]["step"]) == 2
+    assert not again.state.get(frozen)
+
+
+@pytest.mark.parametrize("max_norm", [None, 0.1])
+def test_rounding_does_not_depend_on_who_else_has_a_gradient(max_norm):
+    # Three parameters, the first of them without a gradient at first: one
+    # plan, or two.
+    def start(late):
+        gen = torch.Generator().manual_seed(1)
+        params = [torch.nn.Parameter(torch.randn(77, generator=gen))
+                  for _ in range(3)]
+        opt = AdamW(params, state_bits=8, rounding_seed=5, max_norm=max_norm)
+        for k in range(3):
+            for i, p in enumerate(params):
+                p.grad = None if i == 0 and k < late else torch.randn(
+                    77, generator=torch.Generator().manual_seed(10 * i + k))
+            opt.step()
+        return params, opt
+
+    one, opt = start(0)
+    two, opt2 = start(2)
+    assert len(opt._plans) == 1 and len(opt2._plans) == 2
+    if max_norm is None:  # (the norm is over all that are there)
+        for p, q in zip(one[1:], two[1:]):
+            assert torch.equal(p, q)
+            x, y = opt.state[p], opt2.state[q]
+            assert all(torch.equal(x[k].float(), y[k].float()) for k in x)
+    # In one plan again, and with the same norm bit by bit.
+    merged = copy.deepcopy((two, opt2))
+    for params, optimizer in ((two, opt2), merged):
+        for i, p in enumerate(params):
+            p.grad = torch.full((77,), 0.1 * i + 0.01)
+        optimizer.step()
+    assert len(opt2._plans) == 2 and len(merged[1]._plans) == 1
+    for p, q in zip(two, merged[0]):
+        assert torch.equal(p, q)
+        x, y = opt2.state[p], merged[1].state[q]
+        assert all(torch.equal(x[k].float(), y[k].float()) for k in x)
 
 
 def test_registry():

@@ -561,6 +561,63 @@ def test_a_capture_before_the_first_step_is_refused():
                                rtol=0, atol=1e-5)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_and_a_parameter_that_comes_later(bits):
+    def start():
+        params = [torch.nn.Parameter(t.cuda()) for t in _tensors([70, 300, 5])]
+        opt = AdamW(params, lr=1e-2, state_bits=bits, rounding_seed=3)
+        for p in params[1:]:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        return params, opt
+
+    (params, opt), (plain, opt2) = start(), start()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(4):
+        if k % 2:
+            for own in (params, plain):
+                own[0].grad = torch.full((70,), 0.5, device="cuda")
+            opt.step()
+            opt2.step()
+        else:
+            for own in (params, plain):
+                own[0].grad = None
+            graph.replay()
+            opt2.step()
+        torch.cuda.synchronize()
+        assert [int(opt.state[p]["step"]) for p in params[1:]] == [k + 2] * 2
+        for p, q in zip(params, plain):
+            assert torch.equal(p, q)
+            x, y = opt.state.get(p, {}), opt2.state.get(q, {})
+            assert set(x) == set(y) and all(_equal(x[n], y[n]) for n in x)
+
+
+@pytest.mark.parametrize("sizes", [[33, 5000, 70], [2049, 2300000]])
+def test_places_stand_for_tensors(sizes):
+    # Two plans over parts of a list, against the plan over all of it.
+    out = []
+    for parts in ([range(len(sizes))], [[len(sizes) - 1],
+                                        range(len(sizes) - 1)]):
+        p, g = _cuda(_tensors(sizes)), _cuda(_tensors(sizes, seed=5))
+        state = [_cuda(column) for column in _state8(sizes)]
+        for part in parts:
+            pick = lambda x: [x[i] for i in part]  # noqa: E731
+            steps = torch.zeros(len(part), dtype=torch.int32, device="cuda")
+            ops.adamw_step(ops.adamw8_plan(
+                pick(p), *map(pick, state), steps, seed=9, places=part),
+                pick(g), **HYPER)
+        out.append((p, state))
+    for a, b in zip(out[0][0], out[1][0]):
+        assert torch.equal(a, b)
+    for a, b in zip(out[0][1], out[1][1]):
+        assert all(_equal(x, y) for x, y in zip(a, b))
+    with pytest.raises(RuntimeError, match="places"):
+        ops.adamw8_plan(p, *state, torch.zeros(
+            len(sizes), dtype=torch.int32, device="cuda"), places=[0])
+
+
 def test_parameters_that_moved():
     plan, params, state, steps, grads = _small_plan(32)
     want = _small_plan(32)
