@@ -94,9 +94,10 @@ bool capturing() {
          c10::hip::CaptureStatus::None;
 }
 
-// Tables that a captured graph reads stay for the process's life: a replay
-// after the plan is gone would take addresses from memory that is something
-// else by then. 64 bytes for 1024 elements or 2048. Never destroyed.
+// Tables that a captured graph reads stay for the process's life, and so do the
+// step counts, which an optimizer makes for itself: a replay after the plan is
+// gone would take addresses from memory that is something else by then, and
+// count in it. 64 bytes for 1024 elements or 2048. Never destroyed.
 std::vector<Tensor>& captured_tables() {
   static auto* kept = new std::vector<Tensor>();
   return *kept;
@@ -188,8 +189,8 @@ class Plan {
     const auto stream = current.stream();
     if (capturing()) {
       if (!captured_)
-        for (const Tensor& t : {device_work_, tickets_})
-          captured_tables().push_back(t);
+        for (const Tensor& t : {device_work_, tickets_, steps_})
+          captured_tables().push_back(t.detach());
       captured_ = true;
     } else if (current != laid_out_on_) {
       // The allocator must not give these to others before this step is done.

@@ -55,6 +55,9 @@ class AdamW(torch.optim.Optimizer):
     changed in place, replaced, or cleared (the next step starts from zero
     there). :meth:`load_state_dict` replaces them; it also takes the state of a
     ``torch.optim.AdamW``, or of an ``Adam`` without weight decay (32 bits).
+
+    A captured step goes on with the parameters and states that it was captured
+    with: where these are replaced, it has to be captured again.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,

@@ -618,6 +618,30 @@ def test_places_stand_for_tensors(sizes):
             len(sizes), dtype=torch.int32, device="cuda"), places=[0])
 
 
+def test_counts_of_a_captured_step_stay():
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = AdamW([p], lr=0.5, weight_decay=0.)
+    p.grad = torch.ones(8, device="cuda")
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    kept = dict(opt.state[p])  # the captured step's own, but for the counts
+    at = kept.pop("step").data_ptr()
+    opt.load_state_dict(opt.state_dict())
+    opt.step()
+    # The optimizer counts elsewhere now; that memory is nobody else's.
+    assert opt.state[p]["step"].data_ptr() != at
+    torch.cuda.synchronize()
+    others = [torch.zeros(1, dtype=torch.int32, device="cuda")
+              for _ in range(4096)]
+    assert at not in {t.data_ptr() for t in others}
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(opt.state[p]["step"]) == 2
+    assert not bool(torch.stack(others).any())
+
+
 def test_parameters_that_moved():
     plan, params, state, steps, grads = _small_plan(32)
     want = _small_plan(32)
