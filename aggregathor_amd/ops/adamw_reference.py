@@ -206,12 +206,14 @@ class Plan:
                    "the parameters of a plan are on one device")
             _check(_dense(p), f"parameter {i} of shape {tuple(p.shape)} and "
                    f"strides {p.stride()} does not fill its memory")
+            _check(not p.is_neg(), f"parameter {i} is a view that negates")
             for name, s in (("exp_avg", m[i]), (
                     "exp_avg_root" if bits == 8 else "exp_avg_sq", r[i])):
                 _check(s.dtype == kind,
                        f"{name} {i} is {s.dtype}, expected {kind}")
                 _check(s.device == device, f"{name} {i} is on {s.device}, its "
                        f"parameter on {device}")
+                _check(not s.is_neg(), f"{name} {i} is a view that negates")
                 _check(_same_layout(s, p), f"{name} {i} has another shape or "
                        "other strides than its parameter")
             written += [p, m[i], r[i]]
@@ -249,8 +251,9 @@ class Plan:
         clip = None
         if norm is not None:
             _check(norm.device == device and norm.numel() == 1
-                   and norm.dtype == torch.float32,
-                   "norm is one fp32 number on the parameters' device")
+                   and norm.dtype == torch.float32 and not norm.is_neg(),
+                   "norm is one fp32 number on the parameters' device, and no "
+                   "view that negates")
             self._check_apart(norm, "norm")
             clip = torch.where(norm <= max_norm, torch.ones_like(norm),
                                max_norm / norm).reshape(())

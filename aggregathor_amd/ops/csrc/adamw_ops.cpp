@@ -144,8 +144,10 @@ class Plan {
     adamw::Hyper hyper{lr, beta1, beta2, eps, weight_decay, nullptr, max_norm};
     if (norm) {
       TORCH_CHECK(norm->device() == device && norm->numel() == 1 &&
-                      norm->scalar_type() == torch::kFloat32,
-                  "adamw: norm is one fp32 number on the parameters' device");
+                      norm->scalar_type() == torch::kFloat32 &&
+                      !norm->is_neg(),
+                  "adamw: norm is one fp32 number on the parameters' device, "
+                  "and no view that negates");
       check_apart(*norm, "adamw: norm");
       hyper.norm = norm->data_ptr<float>();
     }
@@ -258,6 +260,8 @@ class Plan {
                 s.scalar_type(), ", expected ", type);
     TORCH_CHECK(s.device() == p.device(), "adamw: ", what, " ", i, " is on ",
                 s.device(), ", its parameter on ", p.device());
+    TORCH_CHECK(!s.is_neg(), "adamw: ", what, " ", i,
+                " is a view that negates");
     TORCH_CHECK(same_layout(s, p), "adamw: ", what, " ", i,
                 " has another shape or other strides than its parameter");
   }
@@ -298,6 +302,8 @@ class Plan {
       TORCH_CHECK(p.is_non_overlapping_and_dense(), "adamw: parameter ", i,
                   " of shape ", p.sizes(), " and strides ", p.strides(),
                   " does not fill its memory");
+      TORCH_CHECK(!p.is_neg(), "adamw: parameter ", i,
+                  " is a view that negates");
       check_state(m_[i], p, state_type, "exp_avg", i);
       check_state(r_[i], p, state_type,
                   bits_ == 8 ? "exp_avg_root" : "exp_avg_sq", i);

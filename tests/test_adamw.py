@@ -382,6 +382,31 @@ def test_parameters_that_moved_into_gaps_are_refused():
         ops.adamw_step(plan, [torch.ones(3)], lr=0.1)
 
 
+def test_views_that_negate():
+    # The imaginary part of a conjugate: its memory holds the opposite numbers.
+    def minus(x):
+        out = torch.complex(torch.zeros_like(x), -x).conj().imag
+        assert out.is_neg() and torch.equal(out, x)
+        return out
+
+    def new():
+        return [torch.ones(1, device="cpu") for _ in range(3)]
+    steps = torch.zeros(1, dtype=torch.int32, device="cpu")
+    for k in range(3):
+        p, m, v = (minus(x) if i == k else x for i, x in enumerate(new()))
+        with pytest.raises(RuntimeError, match="negates"):
+            ops.adamw_plan([p], [m], [v], steps)
+    p, m, v = new()
+    plan = ops.adamw_plan([p], [m], [v], steps)
+    five = torch.full((1,), 5., device="cpu")
+    with pytest.raises(RuntimeError, match="negates"):
+        ops.adamw_step(plan, [five], lr=0.1, norm=minus(five), max_norm=1.)
+    # Gradients are only read: they may be.
+    assert float(ops.grad_norm([minus(five)])) == 5
+    ops.adamw_step(plan, [minus(five)], lr=0.1, beta1=0.5)
+    assert float(m) == 3 and int(steps) == 1
+
+
 def test_16_bit_parameters_refuse_other_gradients():
     p = torch.zeros(8, dtype=torch.bfloat16)
     plan = ops.adamw_plan([p], [torch.zeros(8)], [torch.zeros(8)], _steps(0))
