@@ -11,8 +11,12 @@ With ``g`` the gradient, ``t`` the tensor's number of steps and
 
 A plan holds the tensors of a training run (parameters, states, step counts)
 the way an optimizer does, checked and laid out once; each call of
-:func:`adamw_step` brings the gradients. :class:`aggregathor_amd.optim.AdamW`
-is the optimizer on top.
+:func:`adamw_step` brings the gradients. Laying it out takes longer than a step
+(0.3 ms for ResNet-50 on a GPU): every tensor is checked, and a table of 64
+bytes for each 1024 elements (2048 of large 8-bit states) is sent to the device,
+which is waited for. A step whose tensors have other memory than in the last one
+(``param.data = ...``) does it again. :class:`aggregathor_amd.optim.AdamW` is the
+optimizer on top.
 
 Tensors are dense in any order of their dimensions (contiguous, channels
 last, ...), with any number of elements, zero among them. Parameters are fp32,
@@ -55,7 +59,9 @@ def _ext(tensor):
 def grad_norm(grads):
     """L2 norm over all elements of a tensor, or of all tensors of a list, as one
     fp32 number on their device (nothing waits for it). Squares are summed in 64
-    bits, in an order that the tensors' sizes and places alone set. It is not
+    bits, in an order that the tensors' sizes and places in memory alone set: the
+    same tensors have the same norm every time, equal ones elsewhere may have
+    another last bit (those that lie back to back are read as one). It is not
     differentiable: tensors that need a gradient are refused, but under
     ``torch.no_grad()``."""
     if isinstance(grads, torch.Tensor):

@@ -7,7 +7,11 @@ waits for nothing and can be captured into a graph (a captured
 element, or 2.06 with ``state_bits=8``.
 
 The result is a function of parameters, gradients and states alone, bit by bit:
-ranks that hold the same aggregated gradient keep the same parameters.
+ranks that hold the same aggregated gradient keep the same parameters. With
+clipping, the gradients have to lie alike in memory for that (as views into one
+flat buffer do, which is what the engine has): the norm adds up tensors that lie
+back to back as one, so that its last bit may be another for the same gradients
+in separate memory.
 """
 
 from itertools import chain, starmap, zip_longest
