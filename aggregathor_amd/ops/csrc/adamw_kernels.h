@@ -30,11 +30,13 @@ inline long chunk_of(int bits, long elements) {
 // Tensors of one update launch: their gradients' addresses travel in the
 // kernel's arguments, of which there are 4 KiB.
 constexpr int kMaxTensors = 448;
-// Spans of one norm launch, likewise, the workgroups of one such launch at most
-// (three a CU), and the bytes that one of them reads at a time. Measured for
-// VGG-16's bf16 gradient: 512, 768, 1024, 2048 workgroups 52, 46.7, 47.7, 50.5
-// us; 8192, 16384, 32768 bytes 54, 47.7, 48.8 us.
-constexpr int kMaxSpans = 176;
+// Spans of one norm launch: as many as 4 KiB of arguments hold. (ResNet-50's
+// 161 gradients in separate memory: 24.3 us as one launch, 32.4 us as two, and
+// where one is enough, up to 176 or up to 200 of them made no difference.) The
+// workgroups of one such launch at most (three a CU), and the bytes that one of
+// them reads at a time. Measured for VGG-16's bf16 gradient: 512, 768, 1024, 2048
+// workgroups 52, 46.7, 47.7, 50.5 us; 8192, 16384, 32768 bytes 54, 47.7, 48.8 us.
+constexpr int kMaxSpans = 200;
 constexpr int kNormBlocks = 768;
 constexpr int kNormChunkBytes = 16384;
 

@@ -348,7 +348,9 @@ __device__ __forceinline__ Common common(const Scalars& s, uint32_t key,
 // the last of each of these at one. Counters wrap by themselves to the zero that
 // the next launch needs.
 // Up to 64 of them arrive at one at once: a second arrival would take longer
-// than they wait for each other.
+// than they wait for each other. Measured, one address / 32 and one: the step of
+// 64, 96, 128, 192, 512 workgroups 3.88 / 4.00, 3.96 / 3.96, 4.3 / 4.2, 5.2 / 4.2,
+// 9.7 / 5.6 us, the norm 5.1 / 5.2, 5.3 / 5.1, 5.6 / 5.2, 6.2 / 5.2, 10.2 / 5.8.
 __device__ __forceinline__ unsigned lines() {
   return gridDim.x <= 64 ? 1 : kTicketLines;
 }
@@ -662,6 +664,7 @@ int norm_blocks(const Spans& spans) {
 
 void norm_partials(const Spans& spans, double* partials, unsigned* tickets,
                    float* out, hipStream_t stream) {
+  static_assert(sizeof(Spans) + 3 * sizeof(void*) <= 4096);  // the arguments
   norm_kernel<<<norm_blocks(spans), kBlock, 0, stream>>>(spans, partials,
                                                          tickets, out);
 }

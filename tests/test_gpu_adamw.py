@@ -109,6 +109,17 @@ def test_grad_norm_of_many_and_mixed():
     assert abs(float(ops.grad_norm(grads)) - want) <= 2 * oracle.U * want
 
 
+@pytest.mark.parametrize("count", [176, 199, 200, 201, 400, 401])
+def test_grad_norm_of_separate_tensors(count):
+    # Around one launch's spans, and two's.
+    host = _tensors([1 + 37 * i % 211 for i in range(count)])
+    grads = _packed([t for g in host for t in (g, torch.full((1,), 99.))])[0]
+    want = sum(float(g.double().square().sum()) for g in host) ** .5
+    for _ in range(2):
+        got = float(ops.grad_norm(grads[::2]))  # a gap behind each
+        assert abs(got - want) <= 2 * oracle.U * want
+
+
 def test_grad_norm_extremes():
     for value, n, want in ((0., 5, 0.), (1e30, 4, 2e30), (1e-30, 4, 2e-30),
                            (3e38, 1, 3e38), (math.nan, 3, math.nan),
