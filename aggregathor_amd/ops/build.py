@@ -53,9 +53,11 @@ def _compile_flags():
         f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
         # NaN ordering is load-bearing in every GAR: never fast-math.
         "-fno-fast-math",
-        # No packed fp32 instructions: some of their forms are not reliable
-        # on this hardware. (The host pass does not know the feature and
-        # says so; that is harmless.)
+        # No packed fp32 instructions (v_pk_add_f32 and its kind): some of
+        # their forms have given wrong results on this hardware now and then,
+        # without an error, and the GAR kernels are as fast without them
+        # (profiles/gar_kernels.md). (The host pass does not know the feature
+        # and says so; that is harmless.)
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",

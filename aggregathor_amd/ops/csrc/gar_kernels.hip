@@ -104,8 +104,9 @@ static bool use_mfma_sqdist() {
     const char* e = getenv("AGGREGATHOR_SQDIST");
     if (e && strcmp(e, "mfma") == 0) v = 1;
     else if (e && strcmp(e, "valu") == 0) v = 0;
-    // Default: VALU. Measured on MI355X (n=8, d=25.6M fp32): VALU 0.200 ms
-    // (4.1 TB/s algorithmic) vs MFMA 0.606 ms. The f32-input MFMA runs at
+    // Default: VALU. Measured on MI355X (d=25.6M fp32, built without packed
+    // fp32): n=8 VALU 0.174 ms (4.7 TB/s algorithmic) vs MFMA 0.640 ms, n=11
+    // 0.617 vs 1.95, n=16 0.710 vs 2.12. The f32-input MFMA runs at
     // the f32 VECTOR rate (64 cyc/SIMD issue for 32x32x2, guide section 3)
     // and only the 28-of-1024 diagonal outputs are useful, so the MFMA
     // formulation is ISSUE-bound ~2.5x over HBM at small n, while the VALU
