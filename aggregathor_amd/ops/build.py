@@ -28,6 +28,7 @@ OBJ = OPS_DIR / "_obj"
 SOURCES = [CSRC / "gar_ops.cpp", CSRC / "gar_kernels.hip",
            CSRC / "bn_kernels.hip", CSRC / "adamw_ops.cpp",
            CSRC / "adamw_kernels.hip"]
+FLAGS = pathlib.Path(__file__).resolve()  # how they are compiled
 HEADERS = [CSRC / "gar_kernels.h", CSRC / "adamw_kernels.h"]
 
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
@@ -42,7 +43,8 @@ def needs_build():
     if not OUT.exists():
         return True
     out_mtime = OUT.stat().st_mtime
-    return any(p.stat().st_mtime > out_mtime for p in SOURCES + HEADERS)
+    return any(p.stat().st_mtime > out_mtime
+               for p in SOURCES + HEADERS + [FLAGS])
 
 
 def _compile_flags():
@@ -53,11 +55,10 @@ def _compile_flags():
         f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
         # NaN ordering is load-bearing in every GAR: never fast-math.
         "-fno-fast-math",
-        # No packed fp32 instructions (v_pk_add_f32 and its kind): some of
-        # their forms have given wrong results on this hardware now and then,
-        # without an error, and the GAR kernels are as fast without them
-        # (profiles/gar_kernels.md). (The host pass does not know the feature
-        # and says so; that is harmless.)
+        # No packed fp32 instructions: some of their forms have given wrong
+        # results on this hardware now and then, without an error, and the GAR
+        # kernels are as fast without them (profiles/gar_kernels.md). (The host
+        # pass does not know the feature and says so; that is harmless.)
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",

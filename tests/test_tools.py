@@ -1,5 +1,7 @@
 """Tools layer: parse_keyval, ClassRegister, Checkpoints, Context."""
 
+import os
+
 import pytest
 import torch
 
@@ -73,3 +75,25 @@ def test_context_nesting(capsys):
             tools.info("hello")
     out = capsys.readouterr().out
     assert "[outer] [inner] hello" in out
+
+
+def test_build_sees_what_is_newer(tmp_path, monkeypatch):
+    """A library is out of date once a source, a header or the flags changed."""
+    from aggregathor_amd.ops import build
+    files = {}
+    for name in ("a.hip", "a.h", "build.py", "out.so"):
+        files[name] = tmp_path / name
+        files[name].touch()
+    monkeypatch.setattr(build, "SOURCES", [files["a.hip"]])
+    monkeypatch.setattr(build, "HEADERS", [files["a.h"]])
+    monkeypatch.setattr(build, "FLAGS", files["build.py"], raising=False)
+    monkeypatch.setattr(build, "__file__", str(files["build.py"]))
+    monkeypatch.setattr(build, "OUT", files["out.so"])
+    for name in ("a.hip", "a.h", "build.py"):
+        for other in files.values():
+            os.utime(other, (1000, 1000))
+        assert not build.needs_build()
+        os.utime(files[name], (2000, 2000))
+        assert build.needs_build(), name
+    files["out.so"].unlink()
+    assert build.needs_build()
