@@ -27,9 +27,9 @@
 // another implementation's bit by bit. The quotient takes the hardware's
 // reciprocal, and with 32-bit states the root its square root, which are off by
 // a unit in the last place at most (seen over all normal numbers): with 8-bit
-// states the vector units are as busy as the memory, at 80 instructions an
+// states the vector units are as busy as the memory, at 83 instructions an
 // element for 16 bytes (114 with the full sequences for quotient, root and
-// rounding took 411 us for VGG-16 where this takes 360).
+// rounding took 411 us for VGG-16 where this takes 357).
 
 #include <hip/hip_runtime.h>
 
