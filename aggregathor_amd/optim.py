@@ -1,6 +1,6 @@
 """AdamW over the framework's optimizer kernels (:mod:`aggregathor_amd.ops`).
 
-One launch updates every parameter of a group, whatever their number; step
+One launch updates all parameters of a group (one for each 448 of them); step
 counts, clipping and the rounding's random bits live on the device, so a step
 waits for nothing and can be captured into a graph (a captured
 ``torch.optim.Adam`` needs ``capturable=True`` for that). States take 8 bytes an

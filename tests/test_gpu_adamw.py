@@ -629,6 +629,29 @@ def test_places_stand_for_tensors(sizes):
             len(sizes), dtype=torch.int32, device="cuda"), places=[0])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_replaced_before_a_capture(bits):
+    p = torch.nn.Parameter(torch.ones(70, device="cuda"))
+    opt = AdamW([p], lr=0.5, weight_decay=0., state_bits=bits)
+    p.grad = torch.ones(70, device="cuda")
+    opt.step()
+    opt.state[p]["exp_avg"] = opt.state[p]["exp_avg"].clone()
+    before = p.detach().clone()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, before) and int(opt.state[p]["step"]) == 1
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(opt.state[p]["step"]) == 3 + k
+
+
 def test_counts_of_a_captured_step_stay():
     p = torch.nn.Parameter(torch.ones(8, device="cuda"))
     opt = AdamW([p], lr=0.5, weight_decay=0.)
